@@ -38,6 +38,11 @@ extern "C" {
 #define LAED_E_ALIGN  (-2)
 #define LAED_E_SIZE   (-3)
 
+/* element type of a `const void*` tensor argument (everything else is fp32 / int64 as declared) */
+#define LAED_F32  0
+#define LAED_BF16 1
+#define LAED_F16  2
+
 int         laed_version(void);
 const char* laed_last_error(void);
 
@@ -349,6 +354,55 @@ int laed_attn_pool_bwd(const float* enc, int64_t e_sn, int64_t e_st, const float
                        float* denc, int64_t g_sn, int64_t g_st, void* stream);
 int laed_tanh_fwd(const float* x, float* y, int64_t n, void* stream);
 int laed_tanh_bwd(const float* y, const float* dy, float* dx, int64_t n, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Gated linear recurrence (no counterpart in the reference; beside the GRU above):
+ *   h_t = z_t h_{t-1} + (1 - z_t) x_t,  z_t = sigmoid(f_t),  out_t = h_t
+ * gi holds the pre-activations of one Linear layer, its last dimension (f | x) of 2H: element (t, b, c) at
+ * gi[t*gi_st + b*gi_sb + c]; out and dout [T][B][H], dgi like gi; strides in elements, any order of T and B, last
+ * dimension dense.  gi, out, dout, dgi have the type `dtype`; states (h0, hT, dhT, dh0: [B][H]) are fp32, may be NULL (h0 /
+ * dhT: zeros; hT / dh0: not wanted).  lengths (may be NULL): positions t >= lengths[b] are identity steps -- not read, out and
+ * dgi are zeros there, the state passes (a length <= 0: hT = h0; > T: T).  reverse != 0 runs from t = T-1 down to 0.
+ * T = 0 copies h0 to hT.  hT may be h0 (in place).  tape (may be NULL: no backward pass follows): laed_gated_scan_tape
+ * floats written by the forward and read by the backward call, which runs the steps again from it.
+ * ------------------------------------------------------------------------------------------ */
+int64_t laed_gated_scan_tape(int T, int B, int H);
+int laed_gated_scan_fwd(const void* gi, int64_t gi_st, int64_t gi_sb, const float* h0, const int64_t* lengths,
+                        int T, int B, int H, int dtype, int reverse, void* out, int64_t out_st, int64_t out_sb,
+                        float* hT, float* tape, void* stream);
+int laed_gated_scan_bwd(const void* gi, int64_t gi_st, int64_t gi_sb, const float* tape, const int64_t* lengths,
+                        const void* dout, int64_t dout_st, int64_t dout_sb, const float* dhT, int T, int B, int H,
+                        int dtype, int reverse, void* dgi, int64_t dgi_st, int64_t dgi_sb, float* dh0, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Dropout without a stored mask: y = keep ? x / (1-p) : 0 (+ residual), keep(i) = draw offset + i of stream `seed` >= p,
+ * i = row-major number of the element in the LOGICAL shape [d0][d1][d2] whatever the strides (the decision
+ * laed_dropout_keep_mask puts at place i).  The backward pass is the same call on dy without a residual.  Strides of the
+ * two outer dimensions in elements, the last one dense; residual may be NULL; y may be x or residual with the same strides.
+ * A dropped element is 0 whatever x holds there (NaN and infinities too).  rng (may be NULL): device {seed, offset} as two
+ * 64-bit numbers, used instead of the arguments (a captured graph draws new numbers when they are changed between replays).
+ * ------------------------------------------------------------------------------------------ */
+int laed_dropout(const void* x, int64_t xs0, int64_t xs1, const void* residual, int64_t rs0, int64_t rs1,
+                 void* y, int64_t ys0, int64_t ys1, int64_t d0, int64_t d1, int64_t d2, int dtype, float p,
+                 uint64_t seed, uint64_t offset, const void* rng, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * One token per row of logits [N][V] (row stride ld elements, unit column stride) under filters, from a uniform number:
+ *   y_i = (l_i - max l) / temperature, w_i = e^{y_i}; rank = (l descending, index ascending)
+ *   top_k > 0 keeps ranks < top_k; top_p < 1 keeps, of those, tokens in front of which less than top_p of their mass lies
+ *   (the first one always); min_p > 0 keeps w_i >= min_p; the token is the first in vocabulary order whose cumulative kept
+ *   weight exceeds u * total.
+ * Each setting is one number, or one per row where its *_rows pointer is given (device, [N]).  temperature 0: the first
+ * largest logit (logp 0).  u [N] in [0, 1) (values outside are clamped; NaN = 0) or NULL: draw offset + row of stream
+ * `seed`.  -inf and NaN logits are masked (never drawn); of +inf ones each has weight 1 and all others 0; a row with
+ * nothing left gives id -1, logp -inf.  Per-row values out of range: temperature <= 0 or NaN is greedy, top_k <= 0 and
+ * NaN filters are off, top_p <= 0 keeps one token.  logp (may be NULL): log-probability of the token among the kept ones.
+ * Weights are summed as 64-bit fixed-point numbers: results do not depend on the order of any sum.
+ * ------------------------------------------------------------------------------------------ */
+int laed_sample_rows(const void* logits, int64_t ld, int64_t N, int V, int dtype, const float* u, uint64_t seed, uint64_t offset,
+                     double temperature, const float* temperature_rows, int64_t top_k, const int64_t* top_k_rows,
+                     double top_p, const float* top_p_rows, double min_p, const float* min_p_rows,
+                     int64_t* ids, float* logp, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Adam (torch.optim.Adam defaults; model_bases.py:122-125): in place on p, m, v.  `step` is 1-based.

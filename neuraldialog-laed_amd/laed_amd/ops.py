@@ -966,3 +966,286 @@ class LogSoftmaxKFunction(torch.autograd.Function):
         check(lib.laed_gumbel_latent_bwd(None, None, ptr(log_qy), ptr(_f32c(dlq)), R, k, 1.0, ptr(dlogits), stream()),
               "laed_gumbel_latent_bwd")
         return dlogits
+
+
+# ----------------------------------------------------------------------------------------------
+# operators on fp32 / bf16 / fp16 tensors: gated linear recurrence, dropout without a stored mask, filtered sampling
+# ----------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dtype_code(t, what):
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise _lib.LaedError("%s: expected float32, bfloat16 or float16, got %s" % (what, t.dtype))
+    return code
+
+
+def _one_device(what, first, *others):
+    """`first` and the others (None skipped) on one GPU, which is returned."""
+    for t in (first,) + others:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.LaedError("laed_amd kernels need CUDA (ROCm) tensors; got a CPU tensor (%s)" % what)
+        if t.device != first.device:
+            raise _lib.LaedError("%s: tensors on %s and %s" % (what, first.device, t.device))
+    return first.device
+
+
+def _launch(device, fn, what, *args):
+    """fn(*args, stream) on the tensors' own device, on that device's current stream."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, stream()), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream()), what)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _seed_offset(rng, what):
+    """(seed, offset, device tensor or None) of an `rng` argument: a pair of numbers, or an int64 tensor of two."""
+    if torch.is_tensor(rng):
+        if rng.dtype != I64 or rng.numel() != 2 or not rng.is_contiguous():
+            raise _lib.LaedError("%s: an rng tensor holds int64 (seed, offset)" % what)
+        return 0, 0, rng
+    try:
+        seed, offset = rng
+    except TypeError:
+        raise _lib.LaedError("%s: rng is (seed, offset) or an int64 tensor of both" % what)
+    return int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF, None
+
+
+def _scan_check(gi, h0, lengths):
+    if gi.dim() != 3 or gi.shape[2] % 2:
+        raise _lib.LaedError("gated_scan: gi must be [T,B,2H] (f | x), got %s" % (tuple(gi.shape),))
+    _dtype_code(gi, "gated_scan")
+    T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+    if h0 is not None and tuple(h0.shape) != (B, H):
+        raise _lib.LaedError("gated_scan: h0 must be [B,H] = %s, got %s" % ((B, H), tuple(h0.shape)))
+    if lengths is not None and (lengths.dim() != 1 or lengths.shape[0] != B or lengths.dtype.is_floating_point):
+        raise _lib.LaedError("gated_scan: lengths must be [B] integers")
+    _one_device("gated_scan", gi, h0, lengths)
+    return T, B, H
+
+
+def _scan_fwd(gi, h0, lengths, reverse, taped):
+    T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+    dev = gi.device
+    if gi.stride(0) < gi.stride(1):                                # batch-first memory stays batch-first
+        out = torch.empty((B, T, H), device=dev, dtype=gi.dtype).transpose(0, 1)
+    else:
+        out = torch.empty((T, B, H), device=dev, dtype=gi.dtype)
+    hT = torch.empty((B, H), device=dev, dtype=torch.float32)
+    tape = torch.empty(int(lib.laed_gated_scan_tape(T, B, H)), device=dev, dtype=torch.float32) if taped else None
+    _launch(dev, lib.laed_gated_scan_fwd, "laed_gated_scan_fwd", gi.data_ptr(), gi.stride(0), gi.stride(1), _at(h0), _at(lengths),
+            T, B, H, _DTYPES[gi.dtype], int(reverse), out.data_ptr(), out.stride(0), out.stride(1), hT.data_ptr(), _at(tape))
+    return out, hT, tape
+
+
+class GatedScanFunction(torch.autograd.Function):
+    """gi [T,B,2H], h0 [B,H] fp32 or None -> (out [T,B,H], hT [B,H] fp32); see gated_scan."""
+
+    @staticmethod
+    def forward(ctx, gi, h0, lengths, reverse):
+        out, hT, tape = _scan_fwd(gi, h0, lengths, reverse, True)
+        ctx.save_for_backward(gi, tape, lengths)
+        ctx.reverse, ctx.has_h0 = reverse, h0 is not None
+        ctx.set_materialize_grads(False)
+        return out, hT
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dhT):
+        gi, tape, lengths = ctx.saved_tensors
+        T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+        if dout is not None:
+            dout = dout.to(gi.dtype)
+            if dout.stride(2) != 1 and H > 1:
+                dout = dout.contiguous()
+        dhT = None if dhT is None else _f32c(dhT)
+        dgi = torch.empty_like(gi)
+        dh0 = torch.empty((B, H), device=gi.device, dtype=torch.float32) if ctx.has_h0 and ctx.needs_input_grad[1] else None
+        _launch(gi.device, lib.laed_gated_scan_bwd, "laed_gated_scan_bwd", gi.data_ptr(), gi.stride(0), gi.stride(1), tape.data_ptr(),
+                _at(lengths), _at(dout), 0 if dout is None else dout.stride(0), 0 if dout is None else dout.stride(1), _at(dhT),
+                T, B, H, _DTYPES[gi.dtype], int(ctx.reverse), dgi.data_ptr(), dgi.stride(0), dgi.stride(1), _at(dh0))
+        return dgi, dh0, None, None
+
+
+def gated_scan(gi, h0=None, lengths=None, reverse=False):
+    """Gated linear recurrence over time, h_t = z_t h_{t-1} + (1 - z_t) x_t with z_t = sigmoid(f_t).
+
+    gi [T,B,2H] (fp32, bf16 or fp16): the pre-activations (f | x) of one Linear layer, time-major; any strides over T and B
+    (a batch-first tensor is passed as x.transpose(0, 1) and gives a batch-first result).  h0 [B,H]: initial state, zeros if
+    None; states are fp32 whatever gi's type.  lengths [B] int64: positions t >= lengths[b] are padding -- not read, zeros in
+    the output and the gradients, the state passes them unchanged.  reverse: from the last position to the first.
+    -> (out [T,B,H] in gi's type, hT [B,H] fp32).  Differentiable once in gi and h0."""
+    _scan_check(gi, h0, lengths)
+    if gi.stride(2) != 1:
+        gi = gi.contiguous()
+    if h0 is not None:
+        h0 = _f32c(h0)
+    if lengths is not None:
+        lengths = lengths.to(I64).contiguous()
+    if torch.is_grad_enabled() and (gi.requires_grad or (h0 is not None and h0.requires_grad)):
+        return GatedScanFunction.apply(gi, h0, lengths, bool(reverse))
+    out, hT, _ = _scan_fwd(gi, h0, lengths, bool(reverse), False)
+    return out, hT
+
+
+def gated_scan_step(gi, h, h_out=None):
+    """One token of the recurrence (no tape): gi [B,2H], state h [B,H] fp32 -> (out [B,H] in gi's type, new state [B,H] fp32).
+    h_out: where the new state is written (h itself for an update in place)."""
+    if gi.dim() != 2:
+        raise _lib.LaedError("gated_scan_step: gi must be [B,2H] (f | x), got %s" % (tuple(gi.shape),))
+    _scan_check(gi.unsqueeze(0), h, None)
+    B, H = h.shape
+    for t, name in ((h, "h"), (h_out, "h_out")):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or tuple(t.shape) != (B, H)):
+            raise _lib.LaedError("gated_scan_step: %s must be a contiguous fp32 [B,H] state" % name)
+    dev = _one_device("gated_scan_step", gi, h_out)
+    if gi.stride(1) != 1:
+        gi = gi.contiguous()
+    out = torch.empty((B, H), device=dev, dtype=gi.dtype)
+    if h_out is None:
+        h_out = torch.empty_like(h)
+    _launch(dev, lib.laed_gated_scan_fwd, "laed_gated_scan_fwd", gi.data_ptr(), 0, gi.stride(0), h.data_ptr(), None, 1, B, H,
+            _DTYPES[gi.dtype], 0, out.data_ptr(), 0, H, h_out.data_ptr(), None)
+    return out, h_out
+
+
+def _common_rows(*ts):
+    """The tensors' common shape as [d0, d1, d2] with two element strides each -- dimensions that every tensor lays out as
+    one are merged; None if that takes more than three dimensions or a last dimension is not dense."""
+    shape = list(ts[0].shape)
+    strides = [list(t.stride()) for t in ts]
+    dims = [i for i in range(len(shape)) if shape[i] != 1]
+    merged = []                                                    # [size, stride of each tensor], outermost first
+    for i in dims:
+        now = [s[i] for s in strides]
+        if merged and all(m == n * shape[i] for m, n in zip(merged[-1][1], now)):
+            merged[-1] = [merged[-1][0] * shape[i], now]
+        else:
+            merged.append([shape[i], now])
+    if not merged:
+        merged = [[1, [1] * len(ts)]]
+    if len(merged) > 3 or any(s != 1 for s in merged[-1][1]):
+        return None
+    while len(merged) < 3:
+        merged.insert(0, [1, [0] * len(ts)])
+    return [m[0] for m in merged], [(merged[0][1][k], merged[1][1][k]) for k in range(len(ts))]
+
+
+def _dropout_raw(x, residual, p, rng):
+    seed, offset, rng_t = rng
+    code = _DTYPES[x.dtype]
+    y = torch.empty_like(x)
+    if x.is_contiguous() and (residual is None or residual.is_contiguous()):
+        dims, st = (1, 1, x.numel()), ((0, 0),) * 3
+    else:
+        ts = (x, y) if residual is None else (x, y, residual)
+        got = _common_rows(*ts)
+        if got is None:                                            # no three-dimensional walk fits all of them
+            x, y = x.contiguous(), torch.empty(x.shape, device=x.device, dtype=x.dtype)
+            residual = None if residual is None else residual.contiguous()
+            dims, st = (1, 1, x.numel()), ((0, 0),) * 3
+        else:
+            dims, st = got
+    rs = st[2] if residual is not None and len(st) > 2 else (0, 0)
+    _launch(x.device, lib.laed_dropout, "laed_dropout", x.data_ptr(), st[0][0], st[0][1], _at(residual), rs[0], rs[1],
+            y.data_ptr(), st[1][0], st[1][1], dims[0], dims[1], dims[2], code, p, seed, offset, _at(rng_t))
+    return y
+
+
+class DropoutFunction(torch.autograd.Function):
+    """y = keep ? x / (1-p) : 0 (+ residual); nothing but (seed, offset) is kept for the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p, rng):
+        ctx.p, ctx.rng = p, rng[:2]
+        ctx.save_for_backward(rng[2])
+        return _dropout_raw(x, residual, p, rng)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        dx = _dropout_raw(dy, None, ctx.p, ctx.rng + tuple(ctx.saved_tensors)) if ctx.needs_input_grad[0] else None
+        return dx, (dy if ctx.needs_input_grad[1] else None), None, None
+
+
+def dropout(x, p, rng, residual=None):
+    """Dropout drawn from the counter generator, with no mask in memory: y = keep ? x / (1-p) : 0 (+ residual).
+
+    x: fp32, bf16 or fp16, any shape; residual (optional): same shape and type.  rng = (seed, offset): element i in x's logical
+    order is draw offset + i of stream `seed`, the decision dropout_keep_mask(n, p, seed, offset) stores at place i -- a
+    rank of a data-parallel job passes the offset of its first element; or an int64 device tensor of both numbers, for captured
+    graphs (it must hold the same numbers until the backward pass has run).  p = 1 drops everything; a dropped element is 0
+    even where x is NaN or infinite.  Differentiable once in x and residual."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise _lib.LaedError("dropout: p must lie in [0, 1], got %r" % p)
+    _dtype_code(x, "dropout")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise _lib.LaedError("dropout: residual must have x's shape and type (%s %s, got %s %s)"
+                             % (tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
+    rng = _seed_offset(rng, "dropout")
+    _one_device("dropout", x, residual, rng[2])
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return DropoutFunction.apply(x, residual, p, rng)
+    return _dropout_raw(x, residual, p, rng)
+
+
+def _setting(v, name, N, dtype, lo, hi):
+    """A filter setting as (number, tensor or None): a number in [lo, hi], or [N] values on the device."""
+    if torch.is_tensor(v):
+        if v.dim() != 1 or v.shape[0] != N:
+            raise _lib.LaedError("sample_rows: %s per row must be [N] = [%d], got %s" % (name, N, tuple(v.shape)))
+        return 0, v.to(dtype).contiguous()
+    if not (v >= lo and v <= hi):
+        raise _lib.LaedError("sample_rows: %s must lie in [%s, %s], got %r" % (name, lo, hi, v))
+    return v, None
+
+
+def sample_rows(logits, u=None, rng=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logp=False):
+    """One token per row of logits [N,V] (fp32, bf16 or fp16; any row stride), filtered, from uniform numbers in [0, 1).
+
+    u [N] fp32, or rng = (seed, offset): row r uses draw offset + r of stream `seed`.  Each setting is a number or a [N] tensor:
+    temperature (0: the first largest logit), top_k (0: off), top_p (1: off), min_p (0: off; relative to the largest
+    probability).  Filters apply in that order: the top_k largest logits (ties: lower index first), of those the smallest
+    set of the largest ones that holds top_p of their mass, of those the ones of at least min_p times the largest probability.
+    The token is the first in vocabulary order whose cumulative probability exceeds u.  -inf and NaN are never drawn; a row
+    with nothing else gives -1.  -> ids [N] int64, with return_logp also the token's log-probability among the kept ones
+    [N] fp32.  The same numbers always give the same tokens, however the rows are batched."""
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise _lib.LaedError("sample_rows: logits must be [N,V] with V >= 1, got %s" % (tuple(logits.shape),))
+    code = _dtype_code(logits, "sample_rows")
+    N, V = logits.shape
+    seed = offset = 0
+    if (u is None) == (rng is None):
+        raise _lib.LaedError("sample_rows: either u or rng = (seed, offset) is needed")
+    if u is None:
+        seed, offset, rng_t = _seed_offset(rng, "sample_rows")
+        if rng_t is not None:
+            raise _lib.LaedError("sample_rows: rng is a pair of numbers (pass u for numbers held on the device)")
+    elif u.dtype != torch.float32 or tuple(u.shape) != (N,):
+        raise _lib.LaedError("sample_rows: u must be fp32 [N] = [%d], got %s %s" % (N, u.dtype, tuple(u.shape)))
+    inf = float("inf")
+    t, t_rows = _setting(temperature, "temperature", N, torch.float32, 0.0, inf)
+    if not torch.is_tensor(top_k) and int(top_k) != top_k:
+        raise _lib.LaedError("sample_rows: top_k must be a whole number, got %r" % (top_k,))
+    k, k_rows = _setting(top_k, "top_k", N, I64, 0, 2 ** 63 - 1)
+    p, p_rows = _setting(top_p, "top_p", N, torch.float32, 0.0, 1.0)
+    m, m_rows = _setting(min_p, "min_p", N, torch.float32, 0.0, 1.0)
+    dev = _one_device("sample_rows", logits, u, t_rows, k_rows, p_rows, m_rows)
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if u is not None:
+        u = u.contiguous()
+    ids = torch.empty(N, device=dev, dtype=I64)
+    logp = torch.empty(N, device=dev, dtype=torch.float32) if return_logp else None
+    _launch(dev, lib.laed_sample_rows, "laed_sample_rows", logits.data_ptr(), logits.stride(0), N, V, code, _at(u), seed, offset,
+            float(t), _at(t_rows), min(int(k), V), _at(k_rows), float(p), _at(p_rows), float(m), _at(m_rows), ids.data_ptr(), _at(logp))
+    return (ids, logp) if return_logp else ids
