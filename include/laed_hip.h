@@ -364,15 +364,18 @@ int laed_tanh_bwd(const float* y, const float* dy, float* dx, int64_t n, void* s
  * dhT: zeros; hT / dh0: not wanted).  lengths (may be NULL): positions t >= lengths[b] are identity steps -- not read, out and
  * dgi are zeros there, the state passes (a length <= 0: hT = h0; > T: T).  reverse != 0 runs from t = T-1 down to 0.
  * T = 0 copies h0 to hT.  hT may be h0 (in place).  tape (may be NULL: no backward pass follows): laed_gated_scan_tape
- * floats written by the forward and read by the backward call, which runs the steps again from it.
+ * floats written by the forward and read by the backward call, which runs the steps again from it.  ws: scratch of
+ * laed_gated_scan_workspace floats, 16-byte aligned (0: none is needed, NULL) -- few channels and many steps are split over time.
  * ------------------------------------------------------------------------------------------ */
 int64_t laed_gated_scan_tape(int T, int B, int H);
+int64_t laed_gated_scan_workspace(int T, int B, int H);
 int laed_gated_scan_fwd(const void* gi, int64_t gi_st, int64_t gi_sb, const float* h0, const int64_t* lengths,
                         int T, int B, int H, int dtype, int reverse, void* out, int64_t out_st, int64_t out_sb,
-                        float* hT, float* tape, void* stream);
+                        float* hT, float* tape, float* ws, int64_t ws_floats, void* stream);
 int laed_gated_scan_bwd(const void* gi, int64_t gi_st, int64_t gi_sb, const float* tape, const int64_t* lengths,
                         const void* dout, int64_t dout_st, int64_t dout_sb, const float* dhT, int T, int B, int H,
-                        int dtype, int reverse, void* dgi, int64_t dgi_st, int64_t dgi_sb, float* dh0, void* stream);
+                        int dtype, int reverse, void* dgi, int64_t dgi_st, int64_t dgi_sb, float* dh0,
+                        float* ws, int64_t ws_floats, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Dropout without a stored mask: y = keep ? x / (1-p) : 0 (+ residual), keep(i) = draw offset + i of stream `seed` >= p,

@@ -1032,6 +1032,12 @@ def _scan_check(gi, h0, lengths):
     return T, B, H
 
 
+def _scan_ws(T, B, H, device):
+    """Scratch of one call (from torch's allocator each time: a captured graph keeps its own, two streams never share one)."""
+    n = int(lib.laed_gated_scan_workspace(T, B, H))
+    return torch.empty(n, device=device, dtype=torch.float32) if n else None, n
+
+
 def _scan_fwd(gi, h0, lengths, reverse, taped):
     T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
     dev = gi.device
@@ -1041,8 +1047,10 @@ def _scan_fwd(gi, h0, lengths, reverse, taped):
         out = torch.empty((T, B, H), device=dev, dtype=gi.dtype)
     hT = torch.empty((B, H), device=dev, dtype=torch.float32)
     tape = torch.empty(int(lib.laed_gated_scan_tape(T, B, H)), device=dev, dtype=torch.float32) if taped else None
+    ws, ws_n = _scan_ws(T, B, H, dev)
     _launch(dev, lib.laed_gated_scan_fwd, "laed_gated_scan_fwd", gi.data_ptr(), gi.stride(0), gi.stride(1), _at(h0), _at(lengths),
-            T, B, H, _DTYPES[gi.dtype], int(reverse), out.data_ptr(), out.stride(0), out.stride(1), hT.data_ptr(), _at(tape))
+            T, B, H, _DTYPES[gi.dtype], int(reverse), out.data_ptr(), out.stride(0), out.stride(1), hT.data_ptr(), _at(tape),
+            _at(ws), ws_n)
     return out, hT, tape
 
 
@@ -1069,9 +1077,11 @@ class GatedScanFunction(torch.autograd.Function):
         dhT = None if dhT is None else _f32c(dhT)
         dgi = torch.empty_like(gi)
         dh0 = torch.empty((B, H), device=gi.device, dtype=torch.float32) if ctx.has_h0 and ctx.needs_input_grad[1] else None
+        ws, ws_n = _scan_ws(T, B, H, gi.device)
         _launch(gi.device, lib.laed_gated_scan_bwd, "laed_gated_scan_bwd", gi.data_ptr(), gi.stride(0), gi.stride(1), tape.data_ptr(),
                 _at(lengths), _at(dout), 0 if dout is None else dout.stride(0), 0 if dout is None else dout.stride(1), _at(dhT),
-                T, B, H, _DTYPES[gi.dtype], int(ctx.reverse), dgi.data_ptr(), dgi.stride(0), dgi.stride(1), _at(dh0))
+                T, B, H, _DTYPES[gi.dtype], int(ctx.reverse), dgi.data_ptr(), dgi.stride(0), dgi.stride(1), _at(dh0),
+                _at(ws), ws_n)
         return dgi, dh0, None, None
 
 
@@ -1113,7 +1123,7 @@ def gated_scan_step(gi, h, h_out=None):
     if h_out is None:
         h_out = torch.empty_like(h)
     _launch(dev, lib.laed_gated_scan_fwd, "laed_gated_scan_fwd", gi.data_ptr(), 0, gi.stride(0), h.data_ptr(), None, 1, B, H,
-            _DTYPES[gi.dtype], 0, out.data_ptr(), 0, H, h_out.data_ptr(), None)
+            _DTYPES[gi.dtype], 0, out.data_ptr(), 0, H, h_out.data_ptr(), None, None, 0)
     return out, h_out
 
 

@@ -19,7 +19,10 @@ def gated_scan(gi, h0=None, lengths=None, reverse=False, dout=None, dhT=None):
     k = 6 + 1.5 |f| for the smaller gate, and no more for the larger one (1 - smaller).  A step h' = z h + u x then adds
     (k z |h| + (k + 1) u |x| + |h'|) E to z times the error before it.  Steps grouped in blocks (the state in front of a
     block times the block's product of z, plus the block's own sum) round each of those three quantities once more per
-    level of grouping: a factor of 4 covers three levels."""
+    level of grouping: a factor of 4 covers three levels.
+    Backwards g' = z (g + d): a block of steps computes A g + q with q = z d, each product rounded before the sum, so its
+    error goes by z |g| + z |d| also where g and d cancel (z = 1/2, g = 1, d = -1 + 2^-20: the products 1/2 and -1/2 + 2^-21
+    are off by up to k E / 2 each, the exact result is 2^-21): (k + 1) E z (|g| + |d|) + E |g'|, not k E |g'|."""
     T, B, H2 = gi.shape
     H = H2 // 2
     f, x = gi[:, :, :H], gi[:, :, H:]
@@ -52,7 +55,7 @@ def gated_scan(gi, h0=None, lengths=None, reverse=False, dout=None, dhT=None):
         dx, df, back = u[t] * at, at * d * zu, z[t] * at
         e_dx = u[t] * e_at + (k[t] + 1) * E * np.abs(dx)
         e_df = np.abs(d) * zu * e_at + np.abs(at) * zu * (e_before[t] + E * np.abs(d)) + (2 * k[t] + 3) * E * np.abs(df)
-        e_back = z[t] * e_at + (k[t] + 1) * E * np.abs(back)
+        e_back = z[t] * eg + E * ((k[t] + 1) * z[t] * (np.abs(g) + np.abs(at - g)) + np.abs(back))
         dgi[t, :, :H], dgi[t, :, H:] = np.where(mask[t], df, 0), np.where(mask[t], dx, 0)
         e_dgi[t, :, :H], e_dgi[t, :, H:] = np.where(mask[t], e_df, 0), np.where(mask[t], e_dx, 0)
         g, eg = np.where(mask[t], back, g), np.where(mask[t], e_back, eg)

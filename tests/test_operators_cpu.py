@@ -68,12 +68,16 @@ def test_sample_rows_refusals(ops):
 def test_c_entries_check_their_arguments():
     from laed_amd._lib import lib
     assert lib.laed_gated_scan_tape(0, 4, 4) == 0 and lib.laed_gated_scan_tape(1, 4, 5) >= 20
-    assert lib.laed_gated_scan_fwd(None, 0, 0, None, None, -1, 1, 1, 0, 0, None, 0, 0, None, None, None) == -1
-    assert lib.laed_gated_scan_fwd(None, 0, 0, None, None, 1, 1, 1, 3, 0, None, 0, 0, None, None, None) == -1
-    assert lib.laed_gated_scan_fwd(None, 0, 0, None, None, 1, 1, 1, 0, 0, None, 0, 0, None, None, None) == -1
+    assert lib.laed_gated_scan_fwd(None, 0, 0, None, None, -1, 1, 1, 0, 0, None, 0, 0, None, None, None, 0, None) == -1
+    assert lib.laed_gated_scan_fwd(None, 0, 0, None, None, 1, 1, 1, 3, 0, None, 0, 0, None, None, None, 0, None) == -1
+    assert lib.laed_gated_scan_fwd(None, 0, 0, None, None, 1, 1, 1, 0, 0, None, 0, 0, None, None, None, 0, None) == -1
     assert b"null" in lib.laed_last_error()
-    assert lib.laed_gated_scan_fwd(None, 0, 0, None, None, 5, 0, 4, 0, 0, None, 0, 0, None, None, None) == 0
-    assert lib.laed_gated_scan_bwd(None, 0, 0, None, None, None, 0, 0, None, 1, 1, 1, 0, 0, None, 0, 0, None, None) == -1
+    assert lib.laed_gated_scan_fwd(None, 0, 0, None, None, 5, 0, 4, 0, 0, None, 0, 0, None, None, None, 0, None) == 0
+    assert lib.laed_gated_scan_bwd(None, 0, 0, None, None, None, 0, 0, None, 1, 1, 1, 0, 0, None, 0, 0, None, None, 0, None) == -1
+    one = 16 * (1 << 20)                                           # few channels and a long time axis need scratch
+    assert lib.laed_gated_scan_workspace(40, 60, 512) == 0 and lib.laed_gated_scan_workspace(1 << 20, 1, 8) > 0
+    assert lib.laed_gated_scan_fwd(one, 16, 16, None, None, 1 << 20, 1, 8, 0, 0, one, 8, 8, None, None, None, 0, None) == -1
+    assert b"workspace" in lib.laed_last_error()
     d = lib.laed_dropout
     assert d(None, 0, 0, None, 0, 0, None, 0, 0, 1, 1, 4, 0, 0.5, 0, 0, None, None) == -1
     assert d(None, 0, 0, None, 0, 0, None, 0, 0, 1, 1, 4, 0, 1.5, 0, 0, None, None) == -1
