@@ -301,6 +301,15 @@ int laed_gru_decode_sample(const float* emb, const float* w_ih, const float* w_h
                            const float* u, uint64_t seed, uint64_t row0,
                            float* hbuf, float* xbuf, float* gates, float* logits, int64_t* ids_out, void* stream);
 
+/* Free-running decode through the filters of laed_sample_rows: as laed_gru_decode_greedy but step t draws row r's symbol by
+ * u[t][r] ([max_len][B], replayed), or with u == NULL by number t * 2^32 + row0 + r of stream `seed`. */
+int laed_gru_decode_filtered(const float* emb, const float* w_ih, const float* w_hh, const float* b_ih,
+                             const float* b_hh, const float* proj_w, const float* proj_b, const float* h0,
+                             int B, int E, int H, int V, int max_len, int64_t go_id,
+                             const float* u, uint64_t seed, uint64_t row0, double temperature, int64_t top_k,
+                             double top_p, double min_p, float* hbuf, float* xbuf, float* gates, float* logits,
+                             int64_t* ids_out, void* stream);
+
 /* One decode step at a time, for callers that drive their own loop (decoders.py:152-167 forward_step + :219 topk(1)):
  *   laed_gru_cell_fwd: gates[B][3H] (scratch) = x W_ih^T + b_ih, then the fused recurrent step -> hout[B][H]
  *                      (hout must not alias hprev);

@@ -61,16 +61,19 @@ __global__ __launch_bounds__(256) void gumbel_argmax_rows_kernel(const float* __
     }
 }
 
+// temperature / top-k / top-p / min-p of laed_sample_rows; NULL: Gumbel-max over the whole vocabulary
+struct Filter { double temperature; int64_t top_k; double top_p, min_p; };
+
 int decode_loop(const float* emb, const float* w_ih, const float* w_hh, const float* b_ih, const float* b_hh,
                 const float* proj_w, const float* proj_b, const float* h0, int B, int E, int H, int V, int max_len,
-                int64_t go_id, bool sample, const float* u, uint64_t seed, uint64_t row0,
+                int64_t go_id, bool sample, const Filter* filter, const float* u, uint64_t seed, uint64_t row0,
                 float* hbuf, float* xbuf, float* gates, float* logits, int64_t* ids_out, hipStream_t stream);
 }   // namespace
 
 namespace {
 int decode_loop(const float* emb, const float* w_ih, const float* w_hh, const float* b_ih, const float* b_hh,
                 const float* proj_w, const float* proj_b, const float* h0, int B, int E, int H, int V, int max_len,
-                int64_t go_id, bool sample, const float* u, uint64_t seed, uint64_t row0,
+                int64_t go_id, bool sample, const Filter* filter, const float* u, uint64_t seed, uint64_t row0,
                 float* hbuf, float* xbuf, float* gates, float* logits, int64_t* ids_out, hipStream_t stream) {
     void* stream_ = (void*)stream;
     LAED_CHECK_ARG(B > 0 && E > 0 && H > 0 && V > 0 && max_len > 0, "gru_decode: bad size");
@@ -105,6 +108,11 @@ int decode_loop(const float* emb, const float* w_ih, const float* w_hh, const fl
                                  nullptr, false, stream));
         if (!sample) {
             LAED_TRY(laed_argmax_rows(logits, B, V, ldl, ids_out + (int64_t)(t + 1) * B, stream_));
+        } else if (filter) {
+            // one uniform number per (step, global row): number t * 2^32 + row0 + r of stream `seed`
+            LAED_TRY(laed_sample_rows(logits, ldl, B, V, LAED_F32, u ? u + (int64_t)t * B : nullptr, seed, ((uint64_t)t << 32) + row0,
+                                      filter->temperature, nullptr, filter->top_k, nullptr, filter->top_p, nullptr, filter->min_p, nullptr,
+                                      ids_out + (int64_t)(t + 1) * B, nullptr, stream_));
         } else {
             // RNG stream index of element (step t, global row r, v): ((t * 2^32) + row0 + r) * V + v
             const uint64_t idx0 = (((uint64_t)t << 32) + row0) * (uint64_t)V;
@@ -122,7 +130,7 @@ extern "C" int laed_gru_decode_greedy(const float* emb, const float* w_ih, const
                                       int B, int E, int H, int V, int max_len, int64_t go_id,
                                       float* hbuf, float* xbuf, float* gates, float* logits, int64_t* ids_out,
                                       void* stream) {
-    return decode_loop(emb, w_ih, w_hh, b_ih, b_hh, proj_w, proj_b, h0, B, E, H, V, max_len, go_id, false, nullptr, 0, 0,
+    return decode_loop(emb, w_ih, w_hh, b_ih, b_hh, proj_w, proj_b, h0, B, E, H, V, max_len, go_id, false, nullptr, nullptr, 0, 0,
                        hbuf, xbuf, gates, logits, ids_out, (hipStream_t)stream);
 }
 
@@ -132,7 +140,19 @@ extern "C" int laed_gru_decode_sample(const float* emb, const float* w_ih, const
                                       const float* u, uint64_t seed, uint64_t row0,
                                       float* hbuf, float* xbuf, float* gates, float* logits, int64_t* ids_out,
                                       void* stream) {
-    return decode_loop(emb, w_ih, w_hh, b_ih, b_hh, proj_w, proj_b, h0, B, E, H, V, max_len, go_id, true, u, seed, row0,
+    return decode_loop(emb, w_ih, w_hh, b_ih, b_hh, proj_w, proj_b, h0, B, E, H, V, max_len, go_id, true, nullptr, u, seed, row0,
+                       hbuf, xbuf, gates, logits, ids_out, (hipStream_t)stream);
+}
+
+extern "C" int laed_gru_decode_filtered(const float* emb, const float* w_ih, const float* w_hh, const float* b_ih,
+                                        const float* b_hh, const float* proj_w, const float* proj_b, const float* h0,
+                                        int B, int E, int H, int V, int max_len, int64_t go_id,
+                                        const float* u, uint64_t seed, uint64_t row0, double temperature, int64_t top_k,
+                                        double top_p, double min_p, float* hbuf, float* xbuf, float* gates, float* logits,
+                                        int64_t* ids_out, void* stream) {
+    LAED_CHECK_ARG(temperature >= 0.0 && top_p >= 0.0 && top_p <= 1.0 && min_p >= 0.0 && min_p <= 1.0, "gru_decode: filter out of range");
+    const Filter f = {temperature, top_k, top_p, min_p};
+    return decode_loop(emb, w_ih, w_hh, b_ih, b_hh, proj_w, proj_b, h0, B, E, H, V, max_len, go_id, true, &f, u, seed, row0,
                        hbuf, xbuf, gates, logits, ids_out, (hipStream_t)stream);
 }
 

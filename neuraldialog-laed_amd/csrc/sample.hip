@@ -470,13 +470,16 @@ __device__ __forceinline__ void rank(Shared& sh, const Who& w, const Entry* e, i
     __syncthreads();
 }
 
+// one thread each in draw_few
+__device__ __forceinline__ int few_limit(const Who& w) { return w.nt < FEW ? w.nt : FEW; }
+
 // rank order of the filters: larger logit first, then lower index
 __device__ __forceinline__ u64 rank_of(float l, int i) { return ((u64)key_of(l) << 32) | (unsigned)~i; }
 
 // Narrows (row.tval, row.tidx) to the last element in rank order in front of which less than `want` lies -- elements counted
 // (MASS = false, nothing narrowed before) or their weights (then `share` of the kept mass is wanted).  A histogram over linear
 // bins of the logit finds the bin that holds it; the bin's range of floats picks the candidates in a second pass, and they are
-// ranked in LDS.  A count of at most FEW also collects the elements it keeps (sh.few, sh.nfew) on the way.
+// ranked in LDS.  A count of at most few_limit also collects the elements it keeps (sh.few, sh.nfew) on the way.
 // Returns false, nothing narrowed, where the candidates are too many and BISECTS is false.  sh.hist is zero on entry.
 template <bool MASS, bool BISECTS, typename R>
 __device__ __forceinline__ bool narrow(Shared& sh, const Who& w, Row& row, R& walk, u64 want, double share) {
@@ -507,7 +510,7 @@ __device__ __forceinline__ bool narrow(Shared& sh, const Who& w, Row& row, R& wa
     const int bin = __builtin_amdgcn_readfirstlane(sh.bin);
     // the bin's range of logits, a few floats wider: what lies in it is looked at more closely
     const auto edge = [&](int b, int by) { return nudged(row.md - (MASS ? (b * (double)PER_BIN - 0.5) * row.per_step : b / (double)per_unit), by); };
-    const bool few = !MASS && want <= FEW;
+    const bool few = !MASS && want <= (u64)few_limit(w);
     const float hi = uniform(few || bin == 0 ? row.m : edge(bin, 16)), lo = uniform(bin == NBINS - 1 ? -INFINITY : edge(bin + 1, -16));
     walk.each([&](int i, float l) {
         if ((int)(l >= lo) & (int)(l <= hi) && l > -INFINITY) {
@@ -516,7 +519,7 @@ __device__ __forceinline__ bool narrow(Shared& sh, const Who& w, Row& row, R& wa
                 const unsigned at = atomicAdd(&sh.n, 1u);
                 if (at < CAP) sh.cand[at].rank = rank_of(l, i);
             }
-            if (few && b < bin) sh.few[atomicAdd(&sh.nfew, 1u)].rank = rank_of(l, i);      // fewer than want <= FEW of them
+            if (few && b < bin) sh.few[atomicAdd(&sh.nfew, 1u)].rank = rank_of(l, i);      // fewer than want of them
         }
     });
     __syncthreads();
@@ -645,7 +648,7 @@ __device__ __forceinline__ bool draw_row(Shared& sh, const Who& w, const SampleA
     bool few = false;
     if (k > 0 && k < a.V) {
         if (!narrow<false, BISECTS>(sh, w, row, walk, (u64)k, -1.0)) return false;
-        few = k <= FEW && sh.bin >= 0;
+        few = k <= few_limit(w) && sh.bin >= 0;
         __syncthreads();
         if (!few) {
             clear_bins(sh, w);

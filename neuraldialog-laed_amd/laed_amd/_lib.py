@@ -101,6 +101,8 @@ _SIGS = {
     "laed_gru_cell_fwd": ([_p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _p], _i),
     "laed_proj_argmax": ([_p, _p, _p, _i, _i, _i, _p, _p, _p], _i),
     "laed_gru_decode_greedy": ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i64, _p, _p, _p, _p, _p, _p], _i),
+    "laed_gru_decode_filtered": ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i64, _p, _u64, _u64, _d, _i64, _d, _d,
+                                  _p, _p, _p, _p, _p, _p], _i),
     "laed_gru_decode_sample": ([_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i64, _p, _u64, _u64,
                                 _p, _p, _p, _p, _p, _p], _i),
 }

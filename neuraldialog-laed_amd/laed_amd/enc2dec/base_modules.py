@@ -83,6 +83,69 @@ class GRU(nn.Module):
         return torch.cat([out_f, out_b], dim=2).transpose(0, 1), torch.stack([h_f, h_b], dim=0)
 
 
+class GatedRNN(nn.Module):
+    """Layers of the gated linear recurrence h_t = z_t h_{t-1} + (1 - z_t) x_t with (f | x) = W u_t + b, z = sigmoid(f): the
+    recurrence needs no product per step, so a layer is one product over all positions and one scan (rnn_cell='glr').
+    Beside GRU: the same call contract, batch-first [B,T,E] views of time-major memory, states [layers * dirs,B,H]; dropout
+    acts on each layer's output but the last one's, as nn.GRU's does."""
+
+    def __init__(self, input_size, hidden_size, num_layers=1, batch_first=True, dropout=0.0, bidirectional=False):
+        super(GatedRNN, self).__init__()
+        if not batch_first:
+            raise NotImplementedError("laed_amd.GatedRNN: batch_first=True only, as laed_amd.GRU")
+        from ..nn_lib import Dropout
+        self.input_size, self.hidden_size, self.num_layers = input_size, hidden_size, num_layers
+        self.batch_first, self.dropout, self.bidirectional = True, dropout, bidirectional
+        self.suffixes = [''] + (['_reverse'] if bidirectional else [])
+        for layer in range(num_layers):
+            width = input_size if layer == 0 else hidden_size * len(self.suffixes)
+            for sfx in self.suffixes:
+                self.register_parameter('weight_ih_l%d%s' % (layer, sfx), nn.Parameter(torch.empty(2 * hidden_size, width)))
+                self.register_parameter('bias_ih_l%d%s' % (layer, sfx), nn.Parameter(torch.empty(2 * hidden_size)))
+        stdv = 1.0 / math.sqrt(hidden_size)
+        for w in self.parameters():
+            nn.init.uniform_(w, -stdv, stdv)
+        self.drop = nn.ModuleList(Dropout(dropout, seed=2468 + i) for i in range(num_layers - 1))
+
+    def _gates(self, x_tm, layer, sfx=''):
+        T, B, E = x_tm.shape
+        gi = ops.linear(x_tm.reshape(T * B, E), getattr(self, 'weight_ih_l%d%s' % (layer, sfx)), getattr(self, 'bias_ih_l%d%s' % (layer, sfx)))
+        return gi.view(T, B, 2 * self.hidden_size)
+
+    def _run(self, x_tm, hx, lengths):
+        states = []
+        for layer in range(self.num_layers):
+            outs = []
+            for d, sfx in enumerate(self.suffixes):
+                h0 = None if hx is None else hx[layer * len(self.suffixes) + d]
+                out, hT = ops.gated_scan(self._gates(x_tm, layer, sfx), h0, lengths, reverse=bool(sfx))
+                outs.append(out)
+                states.append(hT)
+            x_tm = outs[0] if len(outs) == 1 else torch.cat(outs, dim=2)
+            if layer + 1 < self.num_layers:
+                x_tm = self.drop[layer](x_tm.transpose(0, 1)).transpose(0, 1)      # numbered batch-first, like the input dropout
+        return x_tm, torch.stack(states)
+
+    def forward_tm(self, x_tm, h0=None):
+        """Time-major entry of a single one-way layer, as GRU.forward_tm: x_tm [T,B,E], h0 [B,H] -> (out [T,B,H], hT [B,H])."""
+        if self.num_layers != 1 or self.bidirectional:
+            raise NotImplementedError("laed_amd.GatedRNN.forward_tm: one layer, one direction")
+        return ops.gated_scan(self._gates(x_tm, 0), h0)
+
+    def forward(self, x, hx=None, lengths=None):
+        """x [B,T,E], hx [layers * dirs,B,H] -> (out [B,T,H * dirs], h_n [layers * dirs,B,H]); lengths [B]: positions behind a
+        sequence's end are skipped (zeros in `out`, the state is the one at its end)."""
+        out, h = self._run(x.transpose(0, 1), hx, lengths)
+        return out.transpose(0, 1), h
+
+    def step(self, x, h):
+        """One token of a single one-way layer, no tape: x [B,E], h [B,H] (updated in place) -> out [B,H]."""
+        if self.num_layers != 1 or self.bidirectional:
+            raise NotImplementedError("laed_amd.GatedRNN.step: one layer, one direction")
+        gi = ops.sgemm(x, self.weight_ih_l0.detach(), transB=True, bias=self.bias_ih_l0.detach())
+        return ops.gated_scan_step(gi, h, h_out=h)[0]
+
+
 class BaseRNN(nn.Module):
     SYM_MASK = PAD
     SYM_EOS = EOS
@@ -108,6 +171,8 @@ class BaseRNN(nn.Module):
         self.input_dropout = nn.Dropout(p=input_dropout_p)
         if rnn_cell.lower() == 'gru':
             self.rnn_cell = GRU
+        elif rnn_cell.lower() == 'glr':
+            self.rnn_cell = GatedRNN
         elif rnn_cell.lower() == 'lstm':
             raise NotImplementedError("laed_amd implements the GRU cell only (the default of all four scripts)")
         else:

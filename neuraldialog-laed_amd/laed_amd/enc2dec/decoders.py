@@ -10,7 +10,7 @@ import torch.nn as nn
 
 from .. import ops, parallel
 from ..nn_lib import Embedding, Linear
-from .base_modules import BaseRNN
+from .base_modules import BaseRNN, GatedRNN
 
 TEACH_FORCE = "teacher_forcing"
 TEACH_GEN = "teacher_gen"
@@ -79,6 +79,8 @@ class DecoderRNN(BaseRNN):
             raise NotImplementedError("decoder attention is off in every LAED script (use_attn=False) and not built")
         if tie_output_embed:
             raise NotImplementedError("tie_output_embed is never enabled by the reference's models")
+        if isinstance(self.rnn, GatedRNN) and n_layers != 1:
+            raise NotImplementedError("DecoderRNN: one layer (every LAED model uses 1)")
         self.output_size = vocab_size if output_size is None else output_size
         self.max_length = max_len
         self.use_attention = use_attention
@@ -95,7 +97,7 @@ class DecoderRNN(BaseRNN):
         # noise control for gen_type='sample' (gumbel_max, base_modules.py:54-67)
         self.sample_seed = 9876
         self.sample_step = 0
-        self.injected_u = None             # tests: uniforms [max_len,B,V] replayed instead of the RNG
+        self.injected_u = None             # tests: uniforms [max_len,B,V] ([max_len,B] with filters) replayed instead of the RNG
 
     def _keep_mask_tm(self, B, T, device):
         """uint8 keep mask in time-major layout [T,B,E]; RNG keyed by the GLOBAL batch row."""
@@ -188,8 +190,31 @@ class DecoderRNN(BaseRNN):
         decoder_outputs = LazyLogProbs(torch.stack(hiddens), self.project, B * K)
         return decoder_outputs, h.unsqueeze(0), ret_dict
 
+    def _generate_gated(self, h, sample, filters, u, seed, row0):
+        """Free-running decode of the gated linear recurrence, one token at a time: ids [L,B], states [L+1,B,H]."""
+        B = h.shape[0]
+        W, bias = self.project.weight.detach(), self.project.bias.detach()
+        hbuf = torch.empty((self.max_length + 1,) + tuple(h.shape), device=h.device, dtype=torch.float32)
+        hbuf[0].copy_(h)
+        h = hbuf[0].clone()
+        ids = torch.empty((self.max_length + 1, B), device=h.device, dtype=torch.int64)
+        ids[0].fill_(int(self.sos_id))
+        for t in range(self.max_length):
+            x = self.embedding(ids[t].view(-1, 1)).reshape(B, -1)
+            out = self.rnn.step(x, h)
+            hbuf[t + 1].copy_(out)
+            if sample:
+                logits = ops.logits_rows(out, W, bias)[:, :self.output_size]
+                ids[t + 1].copy_(ops.sample_rows(logits, None if u is None else u[t], None if u is not None else (seed, (t << 32) + row0),
+                                                 **(filters or {})))
+            else:
+                ids[t + 1].copy_(ops.proj_argmax(out, W, bias))
+        return ids[1:], hbuf
+
     def forward(self, batch_size, inputs=None, init_state=None, attn_context=None, mode=TEACH_FORCE,
-                gen_type='greedy', beam_size=4):
+                gen_type='greedy', beam_size=4, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """gen_type='sample': temperature / top_k / top_p / min_p filter each step's distribution (ops.sample_rows; off by
+        default: Gumbel-max over the whole vocabulary, as the reference draws)."""
         ret_dict = dict()
         if mode == GEN:
             inputs = None
@@ -200,22 +225,31 @@ class DecoderRNN(BaseRNN):
             ret_dict[DecoderRNN.KEY_SEQUENCE] = []
             ret_dict[DecoderRNN.KEY_LENGTH] = [self.max_length] * batch_size
             return decoder_outputs, decoder_hidden, ret_dict
+        gated = isinstance(self.rnn, GatedRNN)
         if gen_type == 'beam':
+            if gated:
+                raise NotImplementedError("beam search runs on the GRU cell only")
             return self._beam_search(batch_size, init_state, beam_size)
         if gen_type not in ('greedy', 'sample'):
             raise ValueError("Unsupported decoding mode")            # decoders.py:237
         with torch.no_grad():
             h0 = init_state[0].detach().contiguous()
             sample = gen_type == 'sample'
+            filters = {'temperature': temperature, 'top_k': top_k, 'top_p': top_p, 'min_p': min_p}
+            if filters == {'temperature': 1.0, 'top_k': 0, 'top_p': 1.0, 'min_p': 0.0}:
+                filters = None
+            elif not sample:
+                raise ValueError("temperature, top_k, top_p and min_p belong to gen_type='sample'")
             u = None
             if sample and self.injected_u is not None:          # tests: replay recorded uniforms [max_len,B,V]
                 u = torch.as_tensor(self.injected_u, dtype=torch.float32).to(h0.device).contiguous()
-            ids, hbuf = ops.decode_greedy(self.embedding.weight.detach(), self.rnn.weight_ih_l0.detach(),
+            seed, row0 = self.sample_seed * 1000003 + self.sample_step, parallel.rank() * batch_size
+            ids, hbuf = self._generate_gated(h0, sample, filters, u, seed, row0) if gated else \
+                ops.decode_greedy(self.embedding.weight.detach(), self.rnn.weight_ih_l0.detach(),
                                           self.rnn.weight_hh_l0.detach(), self.rnn.bias_ih_l0.detach(),
                                           self.rnn.bias_hh_l0.detach(), self.project.weight.detach(),
                                           self.project.bias.detach(), h0, self.max_length, self.sos_id,
-                                          sample=sample, u=u, seed=(self.sample_seed * 1000003 + self.sample_step),
-                                          row0=parallel.rank() * batch_size)
+                                          sample=sample, u=u, seed=seed, row0=row0, filters=filters)
             if sample:
                 self.sample_step += 1
         # ids [L,B]; EOS bookkeeping as decoders.py:241-245 (first EOS position + 1, else max_length)

@@ -42,6 +42,28 @@ class Embedding(nn.Embedding):
         return out.view(T, B, self.embedding_dim).transpose(0, 1)
 
 
+class Dropout(nn.Module):
+    """Dropout drawn inside the kernel, forward and backward each from (seed, step): no mask in memory.  Every call draws the next
+    step's numbers, element i of the GLOBAL batch always the same ones: x is batch-first [B,...] (any strides), and a rank of a
+    data-parallel job draws from its rows' place on (equal shards).  residual: added to the result in the same kernel."""
+
+    def __init__(self, p=0.5, seed=2468):
+        super(Dropout, self).__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError("dropout probability has to be between 0 and 1, but got %r" % p)
+        self.p, self.seed, self.step = float(p), seed, 0
+
+    def forward(self, x, residual=None):
+        if not self.training or self.p == 0.0:
+            return x if residual is None else x + residual
+        rng = (self.seed * 1000003 + self.step, parallel.rank() * x.numel())
+        self.step += 1
+        return ops.dropout(x, self.p, rng, residual=residual)
+
+    def extra_repr(self):
+        return "p=%g, seed=%d" % (self.p, self.seed)
+
+
 class LinearConnector(nn.Module):
     """latent sample -> decoder initial state [1,B,H] (nn_lib.py:138-164)."""
 

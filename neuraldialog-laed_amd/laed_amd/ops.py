@@ -267,9 +267,10 @@ class DenseLogProbsFunction(torch.autograd.Function):
 
 
 def decode_greedy(emb, w_ih, w_hh, b_ih, b_hh, proj_w, proj_b, h0, max_len, go_id, sample=False, u=None, seed=0,
-                  row0=0):
+                  row0=0, filters=None):
     """Free-running decode from h0 [B,H]: greedy, or (sample=True) Gumbel-max sampling with replayed uniforms
-    u [max_len,B,V] or the counter RNG keyed by (seed, step, row0 + row)."""
+    u [max_len,B,V] or the counter RNG keyed by (seed, step, row0 + row).  filters: dict of sample_rows' temperature, top_k,
+    top_p, min_p -- each symbol is then drawn by sample_rows' rule from one uniform number, u [max_len,B] or the counter RNG."""
     B, H = h0.shape
     V, E = emb.shape
     dev = h0.device
@@ -278,6 +279,20 @@ def decode_greedy(emb, w_ih, w_hh, b_ih, b_hh, proj_w, proj_b, h0, max_len, go_i
     gates = torch.empty((B, 3 * H), device=dev, dtype=torch.float32)
     logits = torch.empty((B, proj_ldl(V)), device=dev, dtype=torch.float32)
     ids = torch.empty((max_len + 1, B), device=dev, dtype=I64)
+    if sample and filters is not None:
+        f = dict({"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}, **filters)
+        for name, hi in (("temperature", float("inf")), ("top_k", 2 ** 63 - 1), ("top_p", 1.0), ("min_p", 1.0)):
+            _setting(f[name], name, B, torch.float32, 0, hi)
+        if len(f) != 4 or any(torch.is_tensor(v) for v in f.values()) or int(f["top_k"]) != f["top_k"]:
+            raise _lib.LaedError("decode: filters are numbers for temperature, top_k, top_p and min_p")
+        if u is not None and tuple(u.shape) != (max_len, B):
+            raise ValueError("decode: u must be [max_len, B] = %s, got %s" % ((max_len, B), tuple(u.shape)))
+        check(lib.laed_gru_decode_filtered(ptr(emb), ptr(w_ih), ptr(w_hh), ptr(b_ih), ptr(b_hh), ptr(proj_w), ptr(proj_b),
+                                           ptr(h0), B, E, H, V, int(max_len), int(go_id), ptr(u), int(seed), int(row0),
+                                           float(f["temperature"]), min(int(f["top_k"]), V), float(f["top_p"]), float(f["min_p"]),
+                                           ptr(hbuf), ptr(xbuf), ptr(gates), ptr(logits), ptr(ids, I64), stream()),
+              "laed_gru_decode_filtered")
+        return ids[1:], hbuf
     if sample:
         if u is not None and tuple(u.shape) != (max_len, B, V):
             raise ValueError("decode: u must be [max_len, B, V] = %s, got %s" % ((max_len, B, V), tuple(u.shape)))

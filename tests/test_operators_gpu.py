@@ -406,6 +406,32 @@ def test_sample_ties(ops, V):
             sample_case(ops, logits, uu, **kw)
 
 
+def test_sample_top_k_borders(ops):
+    """Sizes of top_k around the limits at which its tokens are finished by themselves, for both numbers of threads, alone and
+    with the other filters, with distinct and with tied logits."""
+    g = torch.Generator().manual_seed(6)
+    for V in (700, 2000, 5000):
+        logits = torch.randn(300 if V == 2000 else 4, V, generator=g).cuda()
+        logits[1] = (logits[1] * 4).round() / 4
+        u = torch.rand(logits.shape[0], generator=g).cuda()
+        for k in (2, 63, 255, 256, 257, 400, 511, 512, 513, 600, V - 1):
+            sample_case(ops, logits[:4] if V == 2000 and k != 257 else logits, u[:4] if V == 2000 and k != 257 else u, top_k=k)
+            sample_case(ops, logits[:4], u[:4], top_k=k, top_p=0.9, min_p=0.02, temperature=0.8)
+
+
+def test_sample_spread_logits(ops):
+    """Logits spread over hundreds of units and masked by large negative numbers: borders far below the largest one."""
+    g = torch.Generator().manual_seed(9)
+    rows = torch.randn(4, 6000, generator=g) * torch.tensor([10.0, 40.0, 3.0, 3.0])[:, None]
+    rows[2, 1000:] = -1e4
+    rows[3, ::2] = -1e4
+    u = torch.rand(4, generator=g).cuda()
+    for kw in ({"top_k": 50}, {"top_k": 4000}, {"top_k": 2500, "top_p": 0.99}, {"top_p": 0.999}, {"temperature": 20.0, "top_k": 1500, "top_p": 0.9},
+               {"temperature": 50.0, "top_p": 0.7}):
+        sample_case(ops, rows.cuda(), u, **kw)
+        sample_case(ops, rows.cuda(), u, torch.bfloat16, **kw)
+
+
 def test_sample_wide_and_narrow_ranges(ops):
     g = torch.Generator().manual_seed(8)
     V = 20000
