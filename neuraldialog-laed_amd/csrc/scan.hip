@@ -47,9 +47,9 @@ ScanPlan scan_plan(int T, int B, int H) {
     p.waves = (int)cdiv64(T, (int64_t)p.tiles * LSTEP);            // balanced: 65 steps are 2 tiles of 40, not 64 + 1
     if (p.waves < 1) p.waves = 1;
     p.tiles = (int)cdiv64(T, p.waves * LSTEP);
-    // blocks of 64 x 2 channels; 512 of them keep 256 CUs busy
+    // blocks of 64 x 2 channels; 1024 of them keep 256 CUs busy
     const int64_t strips = cdiv64((int64_t)B * H, 128);
-    int64_t segs = strips >= 512 ? 1 : cdiv64(512, strips);
+    int64_t segs = strips >= 512 ? 1 : cdiv64(1024, strips);
     if (segs > p.tiles / 2) segs = p.tiles / 2;                    // a segment is two tiles at least
     if (segs < 1) segs = 1;
     p.seg_tiles = (int)cdiv64(p.tiles, segs);
@@ -222,20 +222,32 @@ __global__ __launch_bounds__(64 * MAXW) void scan_fwd_kernel(ScanArgs a) {
 
 // Folds the segments' (A, b): b of segment s becomes the state in front of it.  Backward: from the last segment to the first.
 template <bool BWD>
-__global__ __launch_bounds__(64) void scan_carry_kernel(float* ws, const float* first, int64_t C, int segs) {
+__global__ __launch_bounds__(64) void scan_carry_kernel(float* __restrict__ ws, const float* __restrict__ first, int64_t C, int segs) {
     const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
     if (c >= C) return;
     float h = first ? first[c] : 0.f;
-    for (int i = 0; i < segs; ++i) {
-        const int64_t at = (int64_t)(2 * (BWD ? segs - 1 - i : i)) * C + c;
-        const float A = ws[at], b = ws[at + C];
-        ws[at + C] = h;
-        h = fmaf(A, h, b);
+    constexpr int AHEAD = 16;                                      // loads in flight; only the products wait for one another
+    for (int i0 = 0; i0 < segs; i0 += AHEAD) {
+        float A[AHEAD], b[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            const int i = i0 + q < segs ? i0 + q : segs - 1;
+            const int64_t at = (int64_t)(2 * (BWD ? segs - 1 - i : i)) * C + c;
+            A[q] = ws[at];
+            b[q] = ws[at + C];
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+            if (i0 + q < segs) {
+                ws[(int64_t)(2 * (BWD ? segs - 1 - i0 - q : i0 + q)) * C + c + C] = h;
+                h = fmaf(A[q], h, b[q]);
+            }
     }
 }
 
+// at most 128 registers: four waves per SIMD, two blocks per CU (131 without the bound: one)
 template <typename T, int VW, bool AGG>
-__global__ __launch_bounds__(64 * MAXW) void scan_bwd_kernel(ScanArgs a) {
+__global__ __launch_bounds__(64 * MAXW, 4) void scan_bwd_kernel(ScanArgs a) {
     __shared__ Chan<VW> sA[2][MAXW][64], sB[2][MAXW][64], sD[2][MAXW][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = a.waves;
     const Lane<VW> me(a, (int64_t)blockIdx.x * 64 + lane);
@@ -390,14 +402,14 @@ void launch_bwd(const ScanArgs& a, hipStream_t stream) {
 }
 template <typename T>
 void dispatch(const ScanArgs& a, bool bwd, hipStream_t stream) {
-    constexpr int es = sizeof(T), wide = 8 / sizeof(T);
+    constexpr int es = sizeof(T), wide = 8 / sizeof(T), narrow = 2;
     auto ok = [&](int vw) {
         return a.H % vw == 0 && rows_on(a.gi, a.gst, a.gsb, vw, es) &&
                (bwd ? rows_on(a.dgi, a.qst, a.qsb, vw, es) && (!a.dout || rows_on(a.dout, a.dst, a.dsb, vw, es))
                     : rows_on(a.out, a.ost, a.osb, vw, es)) &&
                ((uintptr_t)a.h0 | (uintptr_t)a.hT | (uintptr_t)a.tape | (uintptr_t)a.dhT | (uintptr_t)a.dh0 | (uintptr_t)a.ws) % (vw * 4) == 0;
     };
-    if (ok(wide)) bwd ? launch_bwd<T, wide>(a, stream) : launch_fwd<T, wide>(a, stream);
+    if (bwd ? ok(narrow) : ok(wide)) bwd ? launch_bwd<T, narrow>(a, stream) : launch_fwd<T, wide>(a, stream);
     else bwd ? launch_bwd<T, 1>(a, stream) : launch_fwd<T, 1>(a, stream);
 }
 
