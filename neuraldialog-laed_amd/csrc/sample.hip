@@ -21,6 +21,7 @@ constexpr int STEPS = 1024;               // table steps per octave
 constexpr unsigned PER_BIN = 16;          // steps per bin
 constexpr int FAR = 200 * STEPS;          // weights below 2^-200 are 0
 constexpr int MAXW = 16;                  // waves per block
+constexpr int QUEUE = 64 + 4 * 64;        // a wave's worth left over and four elements of every lane
 
 struct SampleArgs {
     const void* logits;
@@ -41,8 +42,10 @@ struct Entry { u64 rank, weight; };
 
 struct Shared {
     double pow2[STEPS];                   // 2^(fb - i / STEPS)
-    u64 hist[NBINS];
-    Entry cand[CAP];
+    union {
+        struct { u64 hist[NBINS]; Entry cand[CAP]; };
+        float queue[MAXW][QUEUE];         // when the filters are done: logits that wait for their weight, by wave
+    };
     u64 before[CAP];
     Entry few[FEW];                       // the tokens of a small top-k
     u64 wsum[MAXW];
@@ -77,11 +80,11 @@ __device__ __forceinline__ double pow2_step(int i) {
 
 // one value for the whole wave, kept in scalar registers: the passes' constants would be spilled as vector registers
 __device__ __forceinline__ float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
-__device__ __forceinline__ double uniform(double x) {
-    const u64 b = (u64)__double_as_longlong(x);
+__device__ __forceinline__ u64 uniform(u64 b) {
     const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(b >> 32));
-    return __longlong_as_double((long long)(((u64)hi << 32) | lo));
+    return ((u64)hi << 32) | lo;
 }
+__device__ __forceinline__ double uniform(double x) { return __longlong_as_double((long long)uniform((u64)__double_as_longlong(x))); }
 
 // what a row's passes need; all of it uniform
 struct Row {
@@ -161,8 +164,9 @@ struct Place {
     int V, shift, nvec, turns, group, wave, lane;                  // turns: vectors per lane; group: a fourth of them, rounded up
     bool infinite;
     __device__ __forceinline__ Place(const T* row, int V_, int waves, int wave_, int lane_) : V(V_), wave(wave_), lane(lane_), infinite(false) {
-        shift = (int)(((uintptr_t)row & 15) / sizeof(T));
-        p = row - shift;
+        const u64 at = uniform((u64)(uintptr_t)row);               // a descriptor in vector registers would be read lane by lane
+        shift = (int)((at & 15) / sizeof(T));
+        p = (const T*)(uintptr_t)(at & ~15ull);
         nvec = (V + shift + VW - 1) / VW;
         turns = ((nvec + waves - 1) / waves + 63) / 64;
         group = (turns + 3) / 4;
@@ -220,6 +224,9 @@ struct Stream : Place<T> {
             }
         }
     }
+    __device__ __forceinline__ void kept_sums(u64 (&sum)[4], const Row& row, float*) {
+        sums(sum, [&](int i, float l) { return row.drawn(l, i); });
+    }
 };
 
 // the row held in registers, NV vectors per thread: read from memory once
@@ -235,7 +242,8 @@ struct Held : Place<T> {
         // all loads first: the whole vectors through a buffer descriptor of exactly their bytes (one 32-bit offset each, 0 for
         // what lies outside), then the row's first and last vector, which may stick out of it, and -inf behind it
         const int whole0 = this->shift ? 1 : 0, whole1 = (this->V + this->shift) / VW, base = this->vec_of(0);
-        const auto rows = __builtin_amdgcn_make_buffer_rsrc((void*)(this->p + whole0 * VW), 0, (whole1 > whole0 ? whole1 - whole0 : 0) * 16, 0x00027000);
+        const auto rows = __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)uniform((u64)(uintptr_t)(this->p + whole0 * VW)), 0,
+                                                            __builtin_amdgcn_readfirstlane((whole1 > whole0 ? whole1 - whole0 : 0) * 16), 0x00027000);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const auto got = __builtin_amdgcn_raw_buffer_load_b128(rows, (base + 64 * j - whole0) * 16, 0, 0);
@@ -274,10 +282,11 @@ struct Held : Place<T> {
 #pragma unroll
             for (int e = 0; e < VW; ++e) v[j].v[e] = laed_from_float<T>(laed_to_float(v[j].v[e]) == INFINITY ? 0.f : -INFINITY);
     }
-    // f(index, logit, group) for this thread's elements.  The empty asm statements keep the compiler from carrying per-element
-    // results (bins, 64-bit copies) from one pass to the next: a register or more per element, spilled, where recomputing
-    // costs a few instructions.
-    template <typename F> __device__ __forceinline__ void each_in_group(F f) {
+    // f(index, logit, group) for this thread's elements, done(group) behind each group (a fourth of NV vectors).  The empty asm
+    // statements keep the compiler from carrying per-element results (bins, 64-bit copies) from one pass to the next: a
+    // register or more per element, spilled, where recomputing costs a few instructions.
+    template <typename F, typename D> __device__ __forceinline__ void each_in_group(F f, D done) {
+        constexpr int G = (NV + 3) / 4;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
 #pragma unroll
@@ -286,20 +295,52 @@ struct Held : Place<T> {
         int base = this->index_of(this->vec_of(0), 0);
         asm volatile("" : "+v"(base));
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
             if (j < this->turns) {
 #pragma unroll
                 for (int e = 0; e < VW; ++e) {
-                    f(base + 64 * VW * j + e, laed_to_float(v[j].v[e]), j / ((NV + 3) / 4));
+                    f(base + 64 * VW * j + e, laed_to_float(v[j].v[e]), j / G, e);
                     if (e & 1) __builtin_amdgcn_sched_barrier(0);          // two elements' weights in flight, not the whole row's
                 }
             }
+            if (j % G == G - 1 || j == NV - 1) done(j / G);
+        }
     }
     template <typename F> __device__ __forceinline__ void each(F f) {
-        each_in_group([&](int i, float l, int) { f(i, l); });
+        each_in_group([&](int i, float l, int, int) { f(i, l); }, [](int) {});
     }
     template <typename W> __device__ __forceinline__ void sums(u64 (&sum)[4], W weight) {
-        each_in_group([&](int i, float l, int g) { sum[g] += weight(i, l); });
+        each_in_group([&](int i, float l, int g, int) { sum[g] += weight(i, l); }, [](int) {});
+    }
+    // sums of row.drawn.  The kept logits are few, and spread: they are packed into the wave's queue, whose 64 next ones are
+    // weighed at a time, so that every lane weighs a kept one (packing costs 6 instructions an element, weighing 20).
+    __device__ __forceinline__ void kept_sums(u64 (&sum)[4], const Row& row, float* queue) {
+        int n = 0;                                                 // uniform
+        u64 acc = 0;
+        const auto weigh = [&](float l) {
+            const double y = row.steps(l);
+            int k;
+            const u64 v = row.weight(y, k);
+            return y <= row.cut ? v : 0;
+        };
+        each_in_group(
+            [&](int i, float l, int, int e) {
+                const bool keep = row.kept(l, i);
+                const u64 mask = __ballot(keep);
+                if (keep) queue[__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, (unsigned)n))] = l;
+                n += __popcll(mask);
+                if (e % 4 == 3)
+                    while (n >= 64) {
+                        n -= 64;
+                        acc += weigh(queue[n + this->lane]);
+                    }
+            },
+            [&](int g) {                                           // what is left in the queue is this group's own
+                if (this->lane < n) acc += weigh(queue[this->lane]);
+                n = 0;
+                sum[g] = acc;
+                acc = 0;
+            });
     }
 };
 
@@ -336,12 +377,11 @@ __device__ __forceinline__ void find_bin(Shared& sh, const Who& w, u64 base, u64
 }
 
 // First element in vocabulary order at which the cumulative weight exceeds share / 2^64 of the whole; its index in sh.result
-// (-1: none).  -> the whole.  Each wave sums four groups of its vectors; the group that holds the element is read again.
+// (-1: none).  -> the whole.  `sums`: this thread's part of the weight of each of the wave's four groups of vectors; the group
+// that holds the element is read again.
 template <typename R, typename W>
-__device__ __forceinline__ u64 locate(Shared& sh, const Who& w, R& row, u64 share, u64 fixed_target, W weight) {
+__device__ __forceinline__ u64 locate(Shared& sh, const Who& w, R& row, u64 (&sums)[4], u64 share, u64 fixed_target, W weight) {
     constexpr int VW = R::VW;
-    u64 sums[4] = {0, 0, 0, 0};
-    row.sums(sums, weight);
 #pragma unroll
     for (int g = 0; g < 4; ++g) sums[g] = wave_sum64(sums[g]);
     __syncthreads();
@@ -443,7 +483,9 @@ __device__ __forceinline__ void bisect(Shared& sh, const Who& w, Row& row, R& wa
     const u64 each = MASS ? row.weight(tie) : 1;                   // > 0: the equal ones' weight crosses `need`
     const u64 stay = (need - above + each - 1) / each;             // that many of them stay
     const auto one = [&](int i, float l) { return (u64)((int)(l == tie) & (int)row.kept(l, i)); };
-    locate(sh, w, walk, 0, stay - 1, one);
+    u64 sums[4] = {0, 0, 0, 0};
+    walk.sums(sums, one);
+    locate(sh, w, walk, sums, 0, stay - 1, one);
     const int hit = sh.result;                                     // -1: all of them
     row.tidx = __builtin_amdgcn_readfirstlane(hit >= 0 ? hit : (row.tval == tie ? row.tidx : 0x7fffffff));
     row.tval = uniform(tie);
@@ -666,7 +708,10 @@ __device__ __forceinline__ bool draw_row(Shared& sh, const Who& w, const SampleA
     if (few) {
         total = draw_few(sh, w, row, p, share);
     } else {
-        total = locate(sh, w, walk, share, 0, [&](int i, float l) { return row.drawn(l, i); });
+        u64 sums[4] = {0, 0, 0, 0};
+        if (row.tval == -INFINITY && mp <= 0.0) walk.sums(sums, [&](int, float l) { return row.weight(l); });      // everything
+        else walk.kept_sums(sums, row, sh.queue[w.wave]);
+        total = locate(sh, w, walk, sums, share, 0, [&](int i, float l) { return row.drawn(l, i); });
     }
     if (w.tid == 0) {
         const int id = sh.result;
