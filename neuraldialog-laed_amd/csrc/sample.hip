@@ -718,7 +718,7 @@ __device__ __forceinline__ bool draw_row(Shared& sh, const Who& w, const SampleA
         a.ids[r] = id;
         if (a.logp) {
             const double l = (double)walk.clean(laed_to_float(((const T*)a.logits + r * a.ld)[id]));
-            a.logp[r] = (float)((l - (double)m) / setting(a.temperature_rows, a.temperature) - (log((double)total) - a.fb * 0.693147180559945309417));
+            a.logp[r] = (float)((l - (double)m) / setting(a.temperature_rows, a.temperature) - log(ldexp((double)total, -a.fb)));      // one token alone: exactly 0
         }
     }
     return true;

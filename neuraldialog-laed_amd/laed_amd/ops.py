@@ -1099,7 +1099,9 @@ class GatedScanFunction(torch.autograd.Function):
                 dout = dout.contiguous()
             do_st, do_sb, _ = dout.stride()
         dhT = None if dhT is None else _f32c(dhT)
-        dgi = torch.empty_like(gi)
+        dgi = torch.empty_like(gi)                                 # gi's own memory order where that is dense
+        if dgi.stride(2) != 1 or 0 in dgi.stride():
+            dgi = torch.empty(gi.shape, device=gi.device, dtype=gi.dtype)
         dh0 = torch.empty((B, H), device=gi.device, dtype=torch.float32) if ctx.needs_input_grad[1] else None
         ws, ws_n = _scan_ws(T, B, H, gi.device)
         _launch(gi.device, lib.laed_gated_scan_bwd, "laed_gated_scan_bwd", gi.data_ptr(), gi.stride(0), gi.stride(1), tape.data_ptr(),
@@ -1132,7 +1134,7 @@ def gated_scan(gi, h0=None, lengths=None, reverse=False):
 
 def gated_scan_step(gi, h, h_out=None):
     """One token of the recurrence (no tape): gi [B,2H], state h [B,H] fp32 -> (out [B,H] in gi's type, new state [B,H] fp32).
-    h_out: where the new state is written (h itself for an update in place)."""
+    h_out: where the new state is written -- h itself for an update in place, or memory that does not overlap it."""
     if gi.dim() != 2:
         raise _lib.LaedError("gated_scan_step: gi must be [B,2H] (f | x), got %s" % (tuple(gi.shape),))
     _scan_check(gi.unsqueeze(0), h, None)
@@ -1146,6 +1148,8 @@ def gated_scan_step(gi, h, h_out=None):
     out = torch.empty((B, H), device=dev, dtype=gi.dtype)
     if h_out is None:
         h_out = torch.empty_like(h)
+    elif 0 < abs(h_out.data_ptr() - h.data_ptr()) < 4 * B * H:
+        raise _lib.LaedError("gated_scan_step: h_out overlaps h without being h")
     _launch(dev, lib.laed_gated_scan_fwd, "laed_gated_scan_fwd", gi.data_ptr(), 0, gi.stride(0), h.data_ptr(), None, 1, B, H,
             _DTYPES[gi.dtype], 0, out.data_ptr(), 0, H, h_out.data_ptr(), None, None, 0)
     return out, h_out

@@ -92,6 +92,28 @@ def test_c_entries_check_their_arguments():
     assert s(None, 4, 0, 4, 0, None, 0, 0, 1.0, None, 0, None, 1.0, None, 0.0, None, None, None, None) == 0
 
 
+def test_library_holds_no_packed_fp32_arithmetic(tmp_path):
+    """Packed fp32 instructions are switched off in the build: none in the built device code."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    sys.path.insert(0, os.path.join(root, "tools"))
+    import check_mfma_hazards as H
+    if not os.path.exists(os.path.join(H.LLVM, "llvm-objdump")):
+        pytest.skip("no llvm-objdump in this image")
+    local = shutil.copy(os.path.join(H.PKG, "liblaed_hip.so"), str(tmp_path / "lib.so"))
+    subprocess.run([os.path.join(H.LLVM, "llvm-objdump"), "--offloading", local], check=True, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
+    parts = [p for p in os.listdir(str(tmp_path)) if p.endswith("gfx950")]
+    assert parts
+    for part in parts:
+        txt = subprocess.run([os.path.join(H.LLVM, "llvm-objdump"), "-d", str(tmp_path / part)], check=True, stdout=subprocess.PIPE,
+                             universal_newlines=True).stdout
+        assert "v_fma_f32" in txt or "v_fmac_f32" in txt or "s_endpgm" in txt
+        assert not any(op in txt for op in ("v_pk_add_f32", "v_pk_mul_f32", "v_pk_fma_f32"))
+
+
 @pytest.mark.parametrize("reverse", [False, True])
 def test_scan_form_gradients_against_differences(reverse):
     rs = np.random.RandomState(3)

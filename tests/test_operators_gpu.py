@@ -193,6 +193,26 @@ def test_scan_step_is_the_scan(ops, dt):
     close(h, want["hT"], want["hT_err"], torch.float32)
 
 
+def test_scan_step_refuses_overlapping_states(ops):
+    from laed_amd._lib import LaedError
+    buf = torch.zeros(5, 8, device="cuda")
+    with pytest.raises(LaedError, match="overlaps"):
+        ops.gated_scan_step(torch.zeros(4, 16, device="cuda"), buf[:4], h_out=buf[1:])
+    with pytest.raises(LaedError, match="contiguous fp32"):
+        ops.gated_scan_step(torch.zeros(4, 16, device="cuda"), buf[:4], h_out=torch.zeros(8, 4, device="cuda").t())
+
+
+def test_scan_of_inputs_expanded_over_time(ops):
+    g1 = torch.randn(1, 3, 16, device="cuda", requires_grad=True)
+    out, hT = ops.gated_scan(g1.expand(30, 3, 16))
+    g = torch.autograd.grad(out.sum(), g1)[0]
+    g2 = g1.detach().repeat(30, 1, 1).requires_grad_(True)
+    want, _ = ops.gated_scan(g2)
+    assert torch.equal(out, want)
+    d = torch.autograd.grad(want.sum(), g2)[0]
+    assert ((g - d.sum(0, keepdim=True)).abs() <= 30 * F.E * d.abs().sum(0, keepdim=True)).all()
+
+
 def test_scan_is_reproducible_and_leaves_neighbours_alone(ops):
     T, B, H = 500, 2, 40
     gi = torch.randn(T, B, 2 * H, device="cuda", requires_grad=True)
@@ -417,6 +437,14 @@ def test_sample_top_k_borders(ops):
         for k in (2, 63, 255, 256, 257, 400, 511, 512, 513, 600, V - 1):
             sample_case(ops, logits[:4] if V == 2000 and k != 257 else logits, u[:4] if V == 2000 and k != 257 else u, top_k=k)
             sample_case(ops, logits[:4], u[:4], top_k=k, top_p=0.9, min_p=0.02, temperature=0.8)
+
+
+def test_sample_certain_tokens_have_log_probability_zero(ops):
+    logits = torch.randn(6, 3000, device="cuda") * 3
+    u = torch.rand(6, device="cuda")
+    for kw in ({"top_k": 1}, {"top_p": 0.0}, {"min_p": 1.0}, {"temperature": 0.0}, {"temperature": 1e-30}, {"top_k": 1, "top_p": 0.5, "temperature": 0.344}):
+        ids, logp = ops.sample_rows(logits, u, return_logp=True, **kw)
+        assert torch.equal(ids, logits.argmax(dim=1)) and (logp == 0).all(), kw
 
 
 def test_sample_spread_logits(ops):
