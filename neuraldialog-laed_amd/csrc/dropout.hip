@@ -2,6 +2,9 @@
 // them again from (seed, offset), so no mask is written, read or kept for the backward pass.
 //   y = keep ? x * 1/(1-p) : 0  (+ residual),   keep(i) = uniform01(seed, offset + i) >= p
 // The draw of logical element i is the one laed_dropout_keep_mask puts at place i: a stored mask and this kernel agree.
+//
+// fp32 is HBM-bound: 163840 x 1024 in 245 us a pass, 5.5 TB/s (one element per thread and turn: 465 us).  16-bit tensors move
+// half as much per draw and are bound by the hash's 64-bit products: 16384 x 1024 bf16 in 21 us, 0.8 elements per picosecond.
 #include "laed_dtypes.h"
 #include <math.h>
 
