@@ -8,7 +8,8 @@
  * INTEGRATION.md); the in-tree binding is neuraldialog-laed_amd/laed_amd/_lib.py.
  *
  * Conventions
- *   - all matrices are dense row-major fp32; token ids / labels are int64 (model_bases.py:53-57).
+ *   - all matrices are dense row-major fp32; token ids / labels are int64 (model_bases.py:53-57).  Only the entries with a
+ *     `dtype` argument (gated_scan, dropout, sample_rows) take fp32, bf16 or fp16 tensors with strides.
  *   - sequence tensors are TIME-MAJOR inside the library: [T][B][*] (flat row = t*B + b).
  *   - every pointer is a DEVICE pointer owned by the caller (the PyTorch caching allocator);
  *     the library allocates nothing and never synchronises the device.

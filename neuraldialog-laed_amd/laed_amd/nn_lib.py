@@ -45,7 +45,8 @@ class Embedding(nn.Embedding):
 class Dropout(nn.Module):
     """Dropout drawn inside the kernel, forward and backward each from (seed, step): no mask in memory.  Every call draws the next
     step's numbers, element i of the GLOBAL batch always the same ones: x is batch-first [B,...] (any strides), and a rank of a
-    data-parallel job draws from its rows' place on (equal shards).  residual: added to the result in the same kernel."""
+    data-parallel job draws from its rows' place on (equal shards).  residual: added to the result in the same kernel.  The step is
+    the host's number: a captured graph would repeat it (there, ops.dropout with its numbers on the device)."""
 
     def __init__(self, p=0.5, seed=2468):
         super(Dropout, self).__init__()

@@ -1135,14 +1135,14 @@ def gated_scan(gi, h0=None, lengths=None, reverse=False):
 def gated_scan_step(gi, h, h_out=None):
     """One token of the recurrence (no tape): gi [B,2H], state h [B,H] fp32 -> (out [B,H] in gi's type, new state [B,H] fp32).
     h_out: where the new state is written -- h itself for an update in place, or memory that does not overlap it."""
-    if gi.dim() != 2:
+    if gi.dim() != 2 or gi.shape[1] % 2:
         raise _lib.LaedError("gated_scan_step: gi must be [B,2H] (f | x), got %s" % (tuple(gi.shape),))
-    _scan_check(gi.unsqueeze(0), h, None)
-    B, H = h.shape
+    code = _dtype_code(gi, "gated_scan_step")
+    B, H = gi.shape[0], gi.shape[1] // 2
     for t, name in ((h, "h"), (h_out, "h_out")):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or tuple(t.shape) != (B, H)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (B, H) or not t.is_contiguous()):
             raise _lib.LaedError("gated_scan_step: %s must be a contiguous fp32 [B,H] state" % name)
-    dev = _one_device("gated_scan_step", gi, h_out)
+    dev = _one_device("gated_scan_step", gi, h, h_out)
     if gi.stride(1) != 1:
         gi = gi.contiguous()
     out = torch.empty((B, H), device=dev, dtype=gi.dtype)
@@ -1151,7 +1151,7 @@ def gated_scan_step(gi, h, h_out=None):
     elif 0 < abs(h_out.data_ptr() - h.data_ptr()) < 4 * B * H:
         raise _lib.LaedError("gated_scan_step: h_out overlaps h without being h")
     _launch(dev, lib.laed_gated_scan_fwd, "laed_gated_scan_fwd", gi.data_ptr(), 0, gi.stride(0), h.data_ptr(), None, 1, B, H,
-            _DTYPES[gi.dtype], 0, out.data_ptr(), 0, H, h_out.data_ptr(), None, None, 0)
+            code, 0, out.data_ptr(), 0, H, h_out.data_ptr(), None, None, 0)
     return out, h_out
 
 

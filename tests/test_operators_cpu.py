@@ -29,8 +29,11 @@ def test_gated_scan_refusals(ops):
     refused("lengths must be", ops.gated_scan, z(2, 3, 4), None, z(3))
     refused("CPU tensor", ops.gated_scan, z(2, 3, 4))
     refused("must be .B,2H", ops.gated_scan_step, z(2, 3, 4), z(3, 2))
-    refused("h0 must be", ops.gated_scan_step, z(3, 4), z(3, 4))
-    refused("CPU tensor|fp32 .B,H. state", ops.gated_scan_step, z(3, 4), z(3, 2, dtype=torch.bfloat16))
+    refused("must be .B,2H", ops.gated_scan_step, z(3, 5), z(3, 2))
+    refused("h must be a contiguous fp32 .B,H. state", ops.gated_scan_step, z(3, 4), z(3, 4))
+    refused("h must be a contiguous fp32 .B,H. state", ops.gated_scan_step, z(3, 4), z(3, 2, dtype=torch.bfloat16))
+    refused("h_out must be", ops.gated_scan_step, z(3, 4), z(3, 2), z(2, 3).t())
+    refused("CPU tensor", ops.gated_scan_step, z(3, 4), z(3, 2))
 
 
 def test_dropout_refusals(ops):
