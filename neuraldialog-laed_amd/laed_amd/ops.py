@@ -1204,13 +1204,19 @@ class DropoutFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, rng):
         ctx.p, ctx.rng = p, rng[:2]
-        ctx.save_for_backward(rng[2])
+        ctx.on_device = rng[2] is not None
+        if ctx.on_device:
+            ctx.save_for_backward(rng[2])
         return _dropout_raw(x, residual, p, rng)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        dx = _dropout_raw(dy, None, ctx.p, ctx.rng + tuple(ctx.saved_tensors)) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:
+            rng = ctx.rng + (ctx.saved_tensors[0] if ctx.on_device else None,)
+            # linear in dy: the same call again where a second derivative is recorded
+            dx = DropoutFunction.apply(dy, None, ctx.p, rng) if torch.is_grad_enabled() and dy.requires_grad else \
+                _dropout_raw(dy, None, ctx.p, rng)
         return dx, (dy if ctx.needs_input_grad[1] else None), None, None
 
 
@@ -1221,7 +1227,7 @@ def dropout(x, p, rng, residual=None):
     order is draw offset + i of stream `seed`, the decision dropout_keep_mask(n, p, seed, offset) stores at place i -- a
     rank of a data-parallel job passes the offset of its first element; or an int64 device tensor of both numbers, for captured
     graphs (it must hold the same numbers until the backward pass has run).  p = 1 drops everything; a dropped element is 0
-    even where x is NaN or infinite.  Differentiable once in x and residual."""
+    even where x is NaN or infinite.  Differentiable in x and residual, twice too."""
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise _lib.LaedError("dropout: p must lie in [0, 1], got %r" % p)

@@ -303,6 +303,18 @@ def test_dropout_numbers_on_the_device(ops):
     assert torch.equal(torch.autograd.grad(y, x, dy)[0], ops.dropout(dy, 0.3, (77, 5)))
 
 
+def test_dropout_second_derivative_and_repeated_backward(ops):
+    x = torch.randn(500, device="cuda", requires_grad=True)
+    for rng in ((8, 1), torch.tensor([8, 1], device="cuda")):
+        y = ops.dropout(x, 0.3, rng)
+        dy = torch.randn(500, device="cuda", requires_grad=True)
+        dx = torch.autograd.grad(y, x, dy, create_graph=True)[0]
+        assert torch.equal(dx, ops.dropout(dy.detach(), 0.3, (8, 1)))
+        v = torch.randn(500, device="cuda")
+        assert torch.equal(torch.autograd.grad(dx, dy, v)[0], ops.dropout(v, 0.3, (8, 1)))
+        assert torch.equal(torch.autograd.grad(y, x, v)[0], ops.dropout(v, 0.3, (8, 1)))
+
+
 def test_dropout_shards_draw_the_whole_batchs_decisions(ops):
     x = torch.randn(8, 50, device="cuda")
     whole = ops.dropout(x, 0.3, (11, 400))
