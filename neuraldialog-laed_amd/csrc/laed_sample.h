@@ -339,14 +339,21 @@ struct Held : Place<T> {
                 const u64 mask = __ballot(keep);
                 if (keep) queue[__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, (unsigned)n))] = l;
                 n += __popcll(mask);
-                if (e % 4 == 3)
+                if (e % 4 == 3) {
+                    // other lanes' entries of the same wave: the LDS takes a wave's accesses in order, the fences keep
+                    // the compiler to it
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     while (n >= 64) {
                         n -= 64;
                         acc += weigh(queue[n + this->lane]);
                     }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                }
             },
             [&](int g) {                                           // what is left in the queue is this group's own
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 if (this->lane < n) acc += weigh(queue[this->lane]);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 n = 0;
                 sum[g] = acc;
                 acc = 0;
@@ -356,10 +363,10 @@ struct Held : Place<T> {
 
 struct Who { int tid, lane, wave, waves, nt; };
 
-// Bins hold weights, best first: finds the first bin at which base + cumulative weight reaches `want` -- or, with share >= 0,
+// Bins hold weights, best first: finds the first bin at which the cumulative weight reaches `want` -- or, with share >= 0,
 // that share of the whole (rounded up, 1 at least) -- and leaves (bin, weight in front of it, want) in shared memory;
 // bin = -1 if the whole is less than `want`.
-__device__ __forceinline__ void find_bin(Shared& sh, const Who& w, u64 base, u64 want, double share) {
+__device__ __forceinline__ void find_bin(Shared& sh, const Who& w, u64 want, double share) {
     const int per = NBINS / w.nt;
     if (w.tid == 0) sh.bin = -1;
     u64 mine = 0;
@@ -367,7 +374,7 @@ __device__ __forceinline__ void find_bin(Shared& sh, const Who& w, u64 base, u64
     const u64 inc = wave_scan64(mine, w.lane);
     if (w.lane == 63) sh.wsum[w.wave] = inc;
     __syncthreads();
-    u64 front = base + inc - mine, whole = 0;
+    u64 front = inc - mine, whole = 0;
     for (int i = 0; i < w.waves; ++i) {
         if (i < w.wave) front += sh.wsum[i];
         whole += sh.wsum[i];
@@ -557,7 +564,7 @@ __device__ __forceinline__ bool narrow(Shared& sh, const Who& w, Row& row, R& wa
         walk.each([&](int i, float l) { if (row.kept(l, i)) atomicAdd(&sh.hist[bin_of(l)], row.weight(l)); });
     }
     __syncthreads();
-    find_bin(sh, w, 0, want, share);
+    find_bin(sh, w, want, share);
     if (sh.bin < 0) return true;                                   // less than `want` in all: everything stays
     const int bin = __builtin_amdgcn_readfirstlane(sh.bin);
     // the bin's range of logits, a few floats wider: what lies in it is looked at more closely
