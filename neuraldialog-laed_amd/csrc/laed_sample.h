@@ -567,10 +567,16 @@ __device__ __forceinline__ bool narrow(Shared& sh, const Who& w, Row& row, R& wa
     find_bin(sh, w, want, share);
     if (sh.bin < 0) return true;                                   // less than `want` in all: everything stays
     const int bin = __builtin_amdgcn_readfirstlane(sh.bin);
-    // the bin's range of logits, a few floats wider: what lies in it is looked at more closely
-    const auto edge = [&](int b, int by) { return nudged(row.md - (MASS ? (b * (double)PER_BIN - 0.5) * row.per_step : b / (double)per_unit), by); };
+    // The candidates are the bin's elements; its range of logits only spares the others the bin's arithmetic.  A bin goes by the
+    // rounded distance from the largest logit (off by half a step of the distance in fp32), and near logit 0 that is far more
+    // than a few floats of the logit: the range is wider by 2^-23 of the distance d, twice that rounding, and, for its own
+    // rounding to fp32, by 16 floats.  side: 1 the upper end of bin b, -1 the lower end of the bin in front of b.
+    const auto edge = [&](int b, int side) {
+        const double d = MASS ? (b * (double)PER_BIN - 0.5) * row.per_step : b / (double)per_unit;
+        return nudged(row.md - d * (1.0 - side * 0x1p-23), 16 * side);
+    };
     const bool few = !MASS && want <= (u64)few_limit(w);
-    const float hi = uniform(few || bin == 0 ? row.m : edge(bin, 16)), lo = uniform(bin == NBINS - 1 ? -INFINITY : edge(bin + 1, -16));
+    const float hi = uniform(few || bin == 0 ? row.m : edge(bin, 1)), lo = uniform(bin == NBINS - 1 ? -INFINITY : edge(bin + 1, -1));
     walk.each([&](int i, float l) {
         if ((int)(l >= lo) & (int)(l <= hi) && l > -INFINITY) {
             const int b = bin_of(l);
@@ -733,7 +739,8 @@ __device__ __forceinline__ bool draw_row(Shared& sh, const Who& w, const SampleA
     if (w.tid == 0) {
         const int id = sh.result;
         a.ids[r] = id;
-        if (a.logp) {
+        if (a.logp && id < 0) a.logp[r] = -INFINITY;               // no element in front of the row is ever read
+        else if (a.logp) {
             const double l = (double)walk.clean(laed_to_float(((const T*)a.logits + r * a.ld)[id]));
             a.logp[r] = (float)((l - (double)m) / setting(a.temperature_rows, a.temperature) - log(ldexp((double)total, -a.fb)));      // one token alone: exactly 0
         }

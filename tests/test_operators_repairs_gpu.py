@@ -1,0 +1,93 @@
+"""gated_scan, dropout, sample_rows and their callers at calls that once went wrong: each against its 64-bit form or definition."""
+import numpy as np
+import pytest
+import torch
+
+import operator_forms as F
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available()
+    from laed_amd import ops as _ops
+    return _ops
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def sample_case(ops, rows, us, **kw):
+    """rows [N,V] fp32 under one setting, every u of `us` for every row: the 64-bit form's tokens, and its log-probabilities to
+    half a step of fp32 and the weights' fixed-point rounding (2^-44 of the largest weight each, V of them)."""
+    N, V = rows.shape
+    host = f64(rows)
+    for u in us:
+        ids, logp = ops.sample_rows(rows.cuda(), torch.full((N,), u, device="cuda"), return_logp=True, **kw)
+        for r in range(N):
+            tok, lp = F.sample_row(host[r], float(np.float32(u)), **kw)
+            assert int(ids[r]) == tok, (r, u, kw, int(ids[r]), tok)
+            assert abs(float(logp[r]) - lp) <= F.E * abs(lp) * 1.01 + V * 2.0 ** -44 + 1e-12, (r, u, kw, float(logp[r]), lp)
+
+
+US = (0.0, 0.3, 0.77, 1.0 - 2.0 ** -24)
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# a border of top-k or of the nucleus far below the largest logit and next to logit 0: the distance from the largest one is
+# rounded by more than the logit itself
+# ----------------------------------------------------------------------------------------------------------------
+def border_rows(V, above, tops, tinies):
+    """Rows with `above` logits from 0.05 to the largest one, the tiny ones next, all others from -1 down; shuffled alike."""
+    rows = []
+    for top in tops:
+        for tiny in tinies:
+            n = V - above - len(tiny)
+            rows.append(torch.cat([torch.linspace(0.05, top, above), torch.tensor(tiny), torch.linspace(-1.0, -3.0, n)]))
+    order = torch.randperm(V, generator=torch.Generator().manual_seed(V))
+    return torch.stack(rows)[:, order]
+
+
+TINY = ([1e-8], [-1e-8], [1e-8, 2e-8, -3e-8, 0.0, 1e-12], [4.7e-7, 3e-9, -4.7e-7, 1e-38], [1e-3, 1e-3 - 1e-9, 1e-3 - 1e-7])
+
+
+@pytest.mark.parametrize("V", [2000, 5000, 30000])
+def test_sample_top_k_border_next_to_zero(ops, V):
+    rows = border_rows(V, 599, (8.0, 20.0, 11.328125), TINY)
+    for k in (598, 599, 600, 601, 602, 604, 606):
+        sample_case(ops, rows, US, top_k=k)
+    sample_case(ops, rows, US[1:3], top_k=601, top_p=0.99, min_p=1e-6, temperature=1.7)
+
+
+def test_sample_top_k_border_is_the_same_in_any_batch(ops):
+    """255 rows of 2000 go to blocks of 1024 threads, 256 of them to blocks of 256: the same tokens, row by row."""
+    rows = border_rows(2000, 599, (8.0,), TINY).repeat(52, 1)[:256].cuda()
+    u = torch.rand(256, generator=torch.Generator().manual_seed(1)).cuda()
+    for k in (300, 599, 600, 601, 603):
+        one, logp1 = ops.sample_rows(rows, u, top_k=k, return_logp=True)
+        two, logp2 = ops.sample_rows(rows[:255], u[:255], top_k=k, return_logp=True)
+        assert torch.equal(one[:255], two) and torch.equal(logp1[:255], logp2) and (one >= 0).all()
+
+
+def test_sample_top_k_border_of_normal_rows(ops):
+    """N(0, 4) rows whose k-th logit lies near 0.1, the largest one near 8."""
+    rows = torch.randn(48, 50000, generator=torch.Generator().manual_seed(11)) * 2
+    for r in range(0, 48, 16):
+        for k in sorted({int((rows[i] > 0.1).sum()) for i in range(r, r + 4)}):
+            sample_case(ops, rows[r:r + 16], (0.4,), top_k=k)
+
+
+@pytest.mark.parametrize("top,bin_", [(8.0, 300), (5.75, 700), (11.3, 1200)])
+def test_sample_nucleus_border_next_to_zero(ops, top, bin_):
+    """The temperature puts a bin's edge within fp64's rounding of logit 0; p crosses inside one of the tiny tokens' weights."""
+    m = float(np.float32(top))
+    tau = m / ((16 * bin_ - 0.5) * np.log(2.0) / 1024)
+    tiny = np.concatenate([s * 10.0 ** np.arange(-18, -12, 0.25) for s in (1, -1)])
+    row = np.concatenate([[m], np.linspace(m - 1, 1, 200), tiny, np.full(100, -5.0)]).astype(np.float32)
+    rows = torch.from_numpy(row)[torch.randperm(len(row), generator=torch.Generator().manual_seed(bin_))][None]
+    y = (np.sort(row.astype(np.float64))[::-1] - m) / tau
+    mass = np.cumsum(np.exp(y))
+    for j in range(200, 200 + len(tiny), 5):
+        sample_case(ops, rows, (0.3, 1.0 - 2.0 ** -24), temperature=tau, top_p=float((mass[j] - np.exp(y[j]) / 2) / mass[-1]))
