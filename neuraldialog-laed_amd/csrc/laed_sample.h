@@ -20,6 +20,7 @@ typedef unsigned long long u64;
 struct SampleArgs {
     const void* logits;
     int64_t ld, N;
+    int64_t row0;                         // first row of this launch
     int V, fb;
     const float* u;
     uint64_t seed, offset;
@@ -753,32 +754,37 @@ template <typename T, typename R, int NT>
 __global__ __launch_bounds__(NT) void sample_rows_kernel(SampleArgs a) {
     __shared__ Shared sh;
     const Who w = {(int)threadIdx.x, (int)threadIdx.x & 63, __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), NT / 64, NT};
+    const int64_t r = a.row0 + blockIdx.x;
     if constexpr (std::is_same<R, Stream<T>>::value) {
-        draw_row<true, T, R>(sh, w, a, blockIdx.x);
-    } else if (!draw_row<false, T, R>(sh, w, a, blockIdx.x)) {
+        draw_row<true, T, R>(sh, w, a, r);
+    } else if (!draw_row<false, T, R>(sh, w, a, r)) {
         __syncthreads();
-        draw_row<true, T, Stream<T>>(sh, w, a, blockIdx.x);
+        draw_row<true, T, Stream<T>>(sh, w, a, r);
     }
 }
 
+// a grid holds fewer than 2^32 threads: more rows than that go in several launches
 template <typename T, typename R, int NT>
-void go(const SampleArgs& a, unsigned grid, hipStream_t stream) {
-    hipLaunchKernelGGL((sample_rows_kernel<T, R, NT>), dim3(grid), dim3(NT), 0, stream, a);
+void go(SampleArgs a, hipStream_t stream) {
+    constexpr int64_t most = (1ll << 31) / NT;
+    for (a.row0 = 0; a.row0 < a.N; a.row0 += most) {
+        const int64_t rows = a.N - a.row0 < most ? a.N - a.row0 : most;
+        hipLaunchKernelGGL((sample_rows_kernel<T, R, NT>), dim3((unsigned)rows), dim3(NT), 0, stream, a);
+    }
 }
 
 template <typename T>
 void launch(const SampleArgs& a, hipStream_t stream) {
-    const unsigned grid = (unsigned)a.N;
     const int64_t nvec = (a.V + 2 * (16 / sizeof(T)) - 2) / (16 / sizeof(T));      // the row's start may lie inside a vector
     // The row in registers, as few vectors a thread as hold it (13 beside 16: 52 registers leave room, 64 spill a little).
     // 256 threads per row where they hold it and rows are many: several rows share a CU and overlap their phases; a few
     // rows are done sooner by 1024.
-    if (nvec <= 512 && (a.N >= 256 || nvec <= 256)) go<T, Held<T, 2>, 256>(a, grid, stream);
-    else if (nvec <= 1024 * 4) go<T, Held<T, 4>, 1024>(a, grid, stream);
-    else if (nvec <= 1024 * 8) go<T, Held<T, 8>, 1024>(a, grid, stream);
-    else if (nvec <= 1024 * 13) go<T, Held<T, 13>, 1024>(a, grid, stream);
-    else if (nvec <= 1024 * 16) go<T, Held<T, 16>, 1024>(a, grid, stream);
-    else go<T, Stream<T>, 1024>(a, grid, stream);
+    if (nvec <= 512 && (a.N >= 256 || nvec <= 256)) go<T, Held<T, 2>, 256>(a, stream);
+    else if (nvec <= 1024 * 4) go<T, Held<T, 4>, 1024>(a, stream);
+    else if (nvec <= 1024 * 8) go<T, Held<T, 8>, 1024>(a, stream);
+    else if (nvec <= 1024 * 13) go<T, Held<T, 13>, 1024>(a, stream);
+    else if (nvec <= 1024 * 16) go<T, Held<T, 16>, 1024>(a, stream);
+    else go<T, Stream<T>, 1024>(a, stream);
 }
 
 }   // namespace

@@ -17,7 +17,7 @@ extern "C" int laed_sample_rows(const void* logits, int64_t ld, int64_t N, int V
     LAED_CHECK_ARG(logits && ids, "sample_rows: null pointer");
     int lg = 0;
     while ((1ll << lg) < V) ++lg;
-    SampleArgs a = {logits, ld, N, V, 62 - lg < 46 ? 62 - lg : 46, u, seed, offset, temperature, temperature_rows, top_k, top_k_rows,
+    SampleArgs a = {logits, ld, N, 0, V, 62 - lg < 46 ? 62 - lg : 46, u, seed, offset, temperature, temperature_rows, top_k, top_k_rows,
                     top_p, top_p_rows, min_p, min_p_rows, ids, logp};
     if (dtype == LAED_BF16) laed_sample_launch_bf16(a, (hipStream_t)stream);
     else if (dtype == LAED_F16) laed_sample_launch_f16(a, (hipStream_t)stream);

@@ -91,3 +91,18 @@ def test_sample_nucleus_border_next_to_zero(ops, top, bin_):
     mass = np.cumsum(np.exp(y))
     for j in range(200, 200 + len(tiny), 5):
         sample_case(ops, rows, (0.3, 1.0 - 2.0 ** -24), temperature=tau, top_p=float((mass[j] - np.exp(y[j]) / 2) / mass[-1]))
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# more work than one grid of fewer than 2^32 threads holds
+# ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("V,N", [(20, (1 << 24) + 5), (2100, (1 << 22) + 3)])
+def test_sample_more_rows_than_a_grid_holds(ops, V, N):
+    """One expanded row drawn from 2^24 times by 256 threads a row, 2^22 times by 1024: what calls of fewer rows draw."""
+    row = torch.randn(1, V, generator=torch.Generator().manual_seed(V)).cuda()
+    ids, logp = ops.sample_rows(row.expand(N, V), rng=(5, 9), temperature=0.7, top_p=0.9, return_logp=True)
+    for lo in range(0, N, 1 << 20):
+        hi = min(lo + (1 << 20), N)
+        part, lpart = ops.sample_rows(row.expand(hi - lo, V), rng=(5, 9 + lo), temperature=0.7, top_p=0.9, return_logp=True)
+        assert torch.equal(ids[lo:hi], part) and torch.equal(logp[lo:hi], lpart), lo
+    assert ids.unique().numel() > 2
