@@ -20,6 +20,7 @@ struct DropArgs {
     unsigned thr;                          // keep <=> 24-bit draw >= thr, thr = ceil(p 2^24)
     uint64_t seed, offset;
     const uint64_t* rng;                   // device (seed, offset), or NULL
+    int64_t block0, last;                  // dense tensors: this launch's first block, and the last one of all
 };
 
 // Elements e0 .. e0 + VW of one row: the generator's index advances by one per element, so its product with the odd constant
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(DropArgs a) {
     const V* x = (const V*)a.x;
     const V* res = (const V*)a.residual;
     V* y = (V*)a.y;
-    const int64_t nv = a.d2 / VW, first = (int64_t)blockIdx.x * (256 * UNITS) + threadIdx.x;
+    const int64_t block = a.block0 + blockIdx.x, nv = a.d2 / VW, first = block * (256 * UNITS) + threadIdx.x;
     V xv[UNITS], rv[UNITS];
 #pragma unroll
     for (int k = 0; k < UNITS; ++k)
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(DropArgs a) {
             drop_vec<T, VW>(xv[k], RES ? &rv[k] : nullptr, yv, key, offset + (uint64_t)(first + k * 256) * VW, a.thr, a.scale);
             y[first + k * 256] = yv;
         }
-    if (VW > 1 && blockIdx.x == gridDim.x - 1 && threadIdx.x < a.d2 - nv * VW) {
+    if (VW > 1 && block == a.last && threadIdx.x < a.d2 - nv * VW) {
         const int64_t i = nv * VW + threadIdx.x;
         laed_vec<T, 1> x1 = {{((const T*)a.x)[i]}}, r1, y1;
         if (RES) r1.v[0] = ((const T*)a.residual)[i];
@@ -98,11 +99,16 @@ __global__ __launch_bounds__(256) void dropout_rows_kernel(DropArgs a) {
 }
 
 template <typename T, int VW>
-void launch(const DropArgs& a, hipStream_t stream) {
+void launch(DropArgs a, hipStream_t stream) {
     if (a.d0 * a.d1 == 1) {
-        const unsigned grid = (unsigned)cdiv64(cdiv64(a.d2, VW), 1024);
-        if (a.residual) hipLaunchKernelGGL((dropout_flat_kernel<T, VW, true>), dim3(grid), dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((dropout_flat_kernel<T, VW, false>), dim3(grid), dim3(256), 0, stream, a);
+        // a grid holds fewer than 2^32 threads: longer tensors (from 2^34 single elements on) go in several launches
+        const int64_t blocks = cdiv64(cdiv64(a.d2, VW), 1024), most = 1 << 23;
+        a.last = blocks - 1;
+        for (a.block0 = 0; a.block0 < blocks; a.block0 += most) {
+            const dim3 grid((unsigned)(blocks - a.block0 < most ? blocks - a.block0 : most));
+            if (a.residual) hipLaunchKernelGGL((dropout_flat_kernel<T, VW, true>), grid, dim3(256), 0, stream, a);
+            else hipLaunchKernelGGL((dropout_flat_kernel<T, VW, false>), grid, dim3(256), 0, stream, a);
+        }
         return;
     }
     const int64_t blocks = cdiv64(a.d0 * a.d1 * (a.d2 / VW), 256);
@@ -136,7 +142,7 @@ extern "C" int laed_dropout(const void* x, int64_t xs0, int64_t xs1, const void*
     LAED_CHECK_ARG(x && y, "dropout: null pointer");
     LAED_CHECK_ARG(d0 <= (1ll << 40) / d1 / d2, "dropout: more than 2^40 elements");
     DropArgs a = {x, residual, y, d0, d1, d2, xs0, xs1, rs0, rs1, ys0, ys1, p < 1.f ? (float)(1.0 / (1.0 - (double)p)) : 0.f,
-                  (unsigned)ceilf(p * 16777216.0f), seed, offset, (const uint64_t*)rng};
+                  (unsigned)ceilf(p * 16777216.0f), seed, offset, (const uint64_t*)rng, 0, 0};
 #define LAUNCH(T) dispatch<T>(a, (hipStream_t)stream)
     LAED_BY_DTYPE(dtype, LAUNCH);
 #undef LAUNCH

@@ -106,3 +106,37 @@ def test_sample_more_rows_than_a_grid_holds(ops, V, N):
         part, lpart = ops.sample_rows(row.expand(hi - lo, V), rng=(5, 9 + lo), temperature=0.7, top_p=0.9, return_logp=True)
         assert torch.equal(ids[lo:hi], part) and torch.equal(logp[lo:hi], lpart), lo
     assert ids.unique().numel() > 2
+
+
+def spare_memory(gib):
+    torch.cuda.empty_cache()
+    return torch.cuda.mem_get_info()[0] > gib * 2.0 ** 30
+
+
+def test_dropout_more_elements_than_a_grid_holds(ops):
+    """2^34 + 5 elements that start off a vector boundary, single elements a thread: 32 GB of bf16, dropped in place."""
+    from laed_amd._lib import check, lib, stream
+    if not spare_memory(48):
+        pytest.skip("needs 48 GB of device memory")
+    n, p = (1 << 34) + 5, 0.25
+    x = torch.ones(n + 2, device="cuda", dtype=torch.bfloat16)
+    at = x[1:].data_ptr()
+    assert at % 16
+    check(lib.laed_dropout(at, 0, 0, None, 0, 0, at, 0, 0, 1, 1, n, 1, p, 7, 3, None, stream()), "laed_dropout")
+    want = torch.tensor(1 / (1 - p), device="cuda").to(torch.bfloat16)
+    for lo in (0, (1 << 33) - 4096, (1 << 34) - 5000, n - 9000):                # the first draws, both launches' ends, the last ones
+        m = min(9000, n - lo)
+        keep = ops.dropout_keep_mask(m, p, 7, 3 + lo, x.device) != 0
+        assert torch.equal(x[1 + lo:1 + lo + m], torch.where(keep, want, torch.zeros_like(want))), lo
+    assert float(x[0]) == 1 and float(x[n + 1]) == 1
+    del x
+    torch.cuda.empty_cache()
+
+
+def test_dropout_lengths_around_a_block(ops):
+    """Remainders of a vector, of a block's 1024 vectors and of both, forward over all of the tensor."""
+    for n in (4095, 4096, 4097, 8191, 8192, 8193, 8195, 12288 + 1):
+        for dt in (torch.float32, torch.bfloat16):
+            x = torch.randn(n, device="cuda").to(dt)
+            keep = ops.dropout_keep_mask(n, 0.5, 3, 4, x.device) != 0
+            assert torch.equal(ops.dropout(x, 0.5, (3, 4)), torch.where(keep, x * 2, torch.zeros_like(x))), (n, dt)
