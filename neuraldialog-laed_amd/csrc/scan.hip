@@ -40,6 +40,7 @@ struct ScanArgs {
     void* dgi; int64_t qst, qsb;
     float* dh0;
     float* ws;                            // segs > 1: [segs][2][B*H], (A, b) of each segment, b replaced by the state in front
+    int64_t strip0;                       // this launch's first strip of 64 lanes
 };
 
 // How time is divided: a function of the sizes alone, so that the backward call finds the forward call's tape.
@@ -142,7 +143,7 @@ template <typename T, int VW, bool AGG>
 __global__ __launch_bounds__(64 * MAXW) void scan_fwd_kernel(ScanArgs a) {
     __shared__ Chan<VW> sA[2][MAXW][64], sB[2][MAXW][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = a.waves;
-    const Lane<VW> me(a, (int64_t)blockIdx.x * 64 + lane);
+    const Lane<VW> me(a, (a.strip0 + blockIdx.x) * 64 + lane);
     const int64_t C = (int64_t)a.B * a.H;
     const int seg = blockIdx.y, tile0 = seg * a.seg_tiles, tile1 = tile0 + a.seg_tiles < a.tiles ? tile0 + a.seg_tiles : a.tiles;
     const T* gi = (const T*)a.gi + me.b * a.gsb + me.k;
@@ -258,7 +259,7 @@ template <typename T, int VW, bool AGG>
 __global__ __launch_bounds__(64 * MAXW, 4) void scan_bwd_kernel(ScanArgs a) {
     __shared__ Chan<VW> sA[2][MAXW][64], sB[2][MAXW][64], sD[2][MAXW][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = a.waves;
-    const Lane<VW> me(a, (int64_t)blockIdx.x * 64 + lane);
+    const Lane<VW> me(a, (a.strip0 + blockIdx.x) * 64 + lane);
     const int64_t C = (int64_t)a.B * a.H;
     const int seg = blockIdx.y, tile0 = seg * a.seg_tiles, tile1 = tile0 + a.seg_tiles < a.tiles ? tile0 + a.seg_tiles : a.tiles;
     const T* gi = (const T*)a.gi + me.b * a.gsb + me.k;
@@ -386,27 +387,30 @@ bool rows_on(const void* p, int64_t st, int64_t sb, int vw, int es) {
     return ((uintptr_t)p % (vw * es)) == 0 && st % vw == 0 && sb % vw == 0;
 }
 
+// a grid holds fewer than 2^32 threads: more strips than that go in several launches
+template <typename F> void over_strips(ScanArgs& a, int vw, F go) {
+    const int64_t strips = cdiv64((int64_t)a.B * a.H, 64 * vw), most = (1ll << 31) / (64 * a.waves);
+    for (a.strip0 = 0; a.strip0 < strips; a.strip0 += most)
+        go(dim3((unsigned)(strips - a.strip0 < most ? strips - a.strip0 : most), a.segs), dim3(64 * a.waves));
+}
+
 template <typename T, int VW>
-void launch_fwd(const ScanArgs& a, hipStream_t stream) {
+void launch_fwd(ScanArgs a, hipStream_t stream) {
     const int64_t C = (int64_t)a.B * a.H;
-    const unsigned strips = (unsigned)cdiv64(C, 64 * VW);
-    const dim3 block(64 * a.waves);
     if (a.segs > 1) {
-        hipLaunchKernelGGL((scan_fwd_kernel<T, VW, true>), dim3(strips, a.segs), block, 0, stream, a);
+        over_strips(a, VW, [&](dim3 grid, dim3 block) { hipLaunchKernelGGL((scan_fwd_kernel<T, VW, true>), grid, block, 0, stream, a); });
         hipLaunchKernelGGL((scan_carry_kernel<false>), dim3((unsigned)cdiv64(C, 64)), dim3(64), 0, stream, a.ws, a.h0, C, a.segs);
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<T, VW, false>), dim3(strips, a.segs), block, 0, stream, a);
+    over_strips(a, VW, [&](dim3 grid, dim3 block) { hipLaunchKernelGGL((scan_fwd_kernel<T, VW, false>), grid, block, 0, stream, a); });
 }
 template <typename T, int VW>
-void launch_bwd(const ScanArgs& a, hipStream_t stream) {
+void launch_bwd(ScanArgs a, hipStream_t stream) {
     const int64_t C = (int64_t)a.B * a.H;
-    const unsigned strips = (unsigned)cdiv64(C, 64 * VW);
-    const dim3 block(64 * a.waves);
     if (a.segs > 1) {
-        hipLaunchKernelGGL((scan_bwd_kernel<T, VW, true>), dim3(strips, a.segs), block, 0, stream, a);
+        over_strips(a, VW, [&](dim3 grid, dim3 block) { hipLaunchKernelGGL((scan_bwd_kernel<T, VW, true>), grid, block, 0, stream, a); });
         hipLaunchKernelGGL((scan_carry_kernel<true>), dim3((unsigned)cdiv64(C, 64)), dim3(64), 0, stream, a.ws, a.dhT, C, a.segs);
     }
-    hipLaunchKernelGGL((scan_bwd_kernel<T, VW, false>), dim3(strips, a.segs), block, 0, stream, a);
+    over_strips(a, VW, [&](dim3 grid, dim3 block) { hipLaunchKernelGGL((scan_bwd_kernel<T, VW, false>), grid, block, 0, stream, a); });
 }
 template <typename T>
 void dispatch(const ScanArgs& a, bool bwd, hipStream_t stream) {

@@ -140,3 +140,26 @@ def test_dropout_lengths_around_a_block(ops):
             x = torch.randn(n, device="cuda").to(dt)
             keep = ops.dropout_keep_mask(n, 0.5, 3, 4, x.device) != 0
             assert torch.equal(ops.dropout(x, 0.5, (3, 4)), torch.where(keep, x * 2, torch.zeros_like(x))), (n, dt)
+
+
+def test_scan_more_channels_than_a_grid_holds(ops):
+    """2^21 sequences x 2049 channels of one bf16 input expanded over the batch, one channel a thread: 2^32 threads and more.
+    Forward and backward; every sequence gives the numbers of a call of four."""
+    if not spare_memory(100):
+        pytest.skip("needs 100 GB of device memory")
+    B, H = 1 << 21, 2049
+    g = torch.Generator(device="cuda").manual_seed(3)
+    gi = torch.randn(1, 1, 2 * H, device="cuda", generator=g).bfloat16()
+    few = gi.expand(1, 4, 2 * H).contiguous().requires_grad_(True)
+    want, wantT = ops.gated_scan(few)
+    dwant = torch.autograd.grad(want, few, torch.ones_like(want))[0]
+    x = gi.expand(1, B, 2 * H).requires_grad_(True)
+    out, hT = ops.gated_scan(x)
+    assert torch.equal(want[0, :1], want[0, 3:]) and torch.equal(dwant[0, :1], dwant[0, 3:])
+    same = lambda a, b: all(bool((a[i:i + (1 << 18)] == b).all()) for i in range(0, B, 1 << 18))   # noqa: E731
+    assert same(out[0], want[0, 0]) and same(hT, wantT[0])
+    del hT
+    d = torch.autograd.grad(out, x, torch.ones(1, 1, H, device="cuda", dtype=torch.bfloat16).expand(1, B, H))[0]
+    assert same(d[0], dwant[0, 0])
+    del out, d, x
+    torch.cuda.empty_cache()
