@@ -1008,6 +1008,17 @@ def _one_device(what, first, *others):
     return dev
 
 
+_forward_ad = torch.autograd.forward_ad
+
+
+def _no_tangents(what, *ts):
+    """Forward-mode derivatives are refused: a kernel would drop the tangent, and a missing one counts as zero."""
+    if getattr(_forward_ad, "_current_level", 0) < 0:              # outside every dual_level: 0.1 us instead of 0.3 a tensor
+        return
+    if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise _lib.LaedError("%s: no forward-mode derivative (torch.autograd.forward_ad) is built" % what)
+
+
 # the current stream's handle as a number: torch.cuda.current_stream() builds a Stream object, 3 us of a 15 us call (15 us in
 # the autograd engine's thread)
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -1092,6 +1103,7 @@ class GatedScanFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dhT):
         gi, tape, lengths = ctx.saved_tensors
+        _no_tangents("gated_scan's backward pass", dout, dhT)
         T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
         do_st = do_sb = 0
         if dout is not None:
@@ -1118,7 +1130,8 @@ def gated_scan(gi, h0=None, lengths=None, reverse=False):
     (a batch-first tensor is passed as x.transpose(0, 1) and gives a batch-first result).  h0 [B,H]: initial state, zeros if
     None; states are fp32 whatever gi's type.  lengths [B] int64: positions t >= lengths[b] are padding -- not read, zeros in
     the output and the gradients, the state passes them unchanged.  reverse: from the last position to the first.
-    -> (out [T,B,H] in gi's type, hT [B,H] fp32).  Differentiable once in gi and h0."""
+    -> (out [T,B,H] in gi's type, hT [B,H] fp32).  Differentiable once in gi and h0, in reverse mode (forward mode is refused)."""
+    _no_tangents("gated_scan", gi, h0)
     _scan_check(gi, h0, lengths)
     if gi.stride(2) != 1:
         gi = gi.contiguous()
@@ -1137,6 +1150,7 @@ def gated_scan_step(gi, h, h_out=None):
     h_out: where the new state is written -- h itself for an update in place, or memory that does not overlap it."""
     if gi.dim() != 2 or gi.shape[1] % 2:
         raise _lib.LaedError("gated_scan_step: gi must be [B,2H] (f | x), got %s" % (tuple(gi.shape),))
+    _no_tangents("gated_scan_step", gi, h)
     code = _dtype_code(gi, "gated_scan_step")
     B, H = gi.shape[0], gi.shape[1] // 2
     for t, name in ((h, "h"), (h_out, "h_out")):
@@ -1212,6 +1226,7 @@ class DropoutFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         dx = None
+        _no_tangents("dropout's backward pass", dy)
         if ctx.needs_input_grad[0]:
             rng = ctx.rng + (ctx.saved_tensors[0] if ctx.on_device else None,)
             # linear in dy: the same call again where a second derivative is recorded
@@ -1227,7 +1242,8 @@ def dropout(x, p, rng, residual=None):
     order is draw offset + i of stream `seed`, the decision dropout_keep_mask(n, p, seed, offset) stores at place i -- a
     rank of a data-parallel job passes the offset of its first element; or an int64 device tensor of both numbers, for captured
     graphs (it must hold the same numbers until the backward pass has run).  p = 1 drops everything; a dropped element is 0
-    even where x is NaN or infinite.  Differentiable in x and residual, twice too."""
+    even where x is NaN or infinite.  Differentiable in x and residual, twice too, in reverse mode (forward mode is refused)."""
+    _no_tangents("dropout", x, residual)
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise _lib.LaedError("dropout: p must lie in [0, 1], got %r" % p)
@@ -1266,6 +1282,8 @@ def sample_rows(logits, u=None, rng=None, temperature=1.0, top_k=0, top_p=1.0, m
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise _lib.LaedError("sample_rows: logits must be [N,V] with V >= 1, got %s" % (tuple(logits.shape),))
     code = _dtype_code(logits, "sample_rows")
+    if return_logp:
+        _no_tangents("sample_rows", logits)
     N, V = logits.shape
     seed = offset = 0
     if (u is None) == (rng is None):

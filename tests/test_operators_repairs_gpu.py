@@ -163,3 +163,20 @@ def test_scan_more_channels_than_a_grid_holds(ops):
     assert same(d[0], dwant[0, 0])
     del out, d, x
     torch.cuda.empty_cache()
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# derivatives
+# ----------------------------------------------------------------------------------------------------------------
+def test_forward_mode_through_a_backward_pass_is_refused(ops):
+    """A gradient that carries a tangent (forward over reverse) is refused as an input that carries one is."""
+    import torch.autograd.forward_ad as forward_ad
+    gi, x = torch.randn(4, 2, 6, device="cuda", requires_grad=True), torch.randn(30, device="cuda", requires_grad=True)
+    with forward_ad.dual_level():
+        for y, leaf in ((ops.gated_scan(gi)[0], gi), (ops.dropout(x, 0.5, (1, 2)), x)):
+            d = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, d, retain_graph=True)
+            assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].shape == leaf.shape
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.dropout(forward_ad.make_dual(x.detach(), torch.ones_like(x)), 0.5, (1, 2))
