@@ -139,9 +139,11 @@ class GatedRNN(nn.Module):
         return out.transpose(0, 1), h
 
     def step(self, x, h):
-        """One token of a single one-way layer, no tape: x [B,E], h [B,H] (updated in place) -> out [B,H]."""
+        """One token of a single one-way layer: x [B,E], h [B,H] (updated in place) -> out [B,H].  No tape, the weights are taken
+        as constants: an x or h that requires grad is refused while gradients are recorded (forward_tm of T = 1 records them)."""
         if self.num_layers != 1 or self.bidirectional:
             raise NotImplementedError("laed_amd.GatedRNN.step: one layer, one direction")
+        ops.refuse_graph("GatedRNN.step", x, h)
         gi = ops.sgemm(x, self.weight_ih_l0.detach(), transB=True, bias=self.bias_ih_l0.detach())
         return ops.gated_scan_step(gi, h, h_out=h)[0]
 

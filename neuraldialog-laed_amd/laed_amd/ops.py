@@ -1019,6 +1019,12 @@ def _no_tangents(what, *ts):
         raise _lib.LaedError("%s: no forward-mode derivative (torch.autograd.forward_ad) is built" % what)
 
 
+def refuse_graph(what, *ts):
+    """Results that no backward pass can reach are refused for inputs that ask for one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise _lib.LaedError("%s has no backward pass: call it under torch.no_grad() or with detached tensors" % what)
+
+
 # the current stream's handle as a number: torch.cuda.current_stream() builds a Stream object, 3 us of a 15 us call (15 us in
 # the autograd engine's thread)
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -1147,10 +1153,12 @@ def gated_scan(gi, h0=None, lengths=None, reverse=False):
 
 def gated_scan_step(gi, h, h_out=None):
     """One token of the recurrence (no tape): gi [B,2H], state h [B,H] fp32 -> (out [B,H] in gi's type, new state [B,H] fp32).
-    h_out: where the new state is written -- h itself for an update in place, or memory that does not overlap it."""
+    h_out: where the new state is written -- h itself for an update in place, or memory that does not overlap it.  Not
+    differentiable: inputs that require grad are refused while gradients are recorded (gated_scan of T = 1 is)."""
     if gi.dim() != 2 or gi.shape[1] % 2:
         raise _lib.LaedError("gated_scan_step: gi must be [B,2H] (f | x), got %s" % (tuple(gi.shape),))
     _no_tangents("gated_scan_step", gi, h)
+    refuse_graph("gated_scan_step", gi, h, h_out)
     code = _dtype_code(gi, "gated_scan_step")
     B, H = gi.shape[0], gi.shape[1] // 2
     for t, name in ((h, "h"), (h_out, "h_out")):
@@ -1278,12 +1286,14 @@ def sample_rows(logits, u=None, rng=None, temperature=1.0, top_k=0, top_p=1.0, m
     set of the largest ones that holds top_p of their mass, of those the ones of at least min_p times the largest probability.
     The token is the first in vocabulary order whose cumulative probability exceeds u.  -inf and NaN are never drawn; a row
     with nothing else gives -1.  -> ids [N] int64, with return_logp also the token's log-probability among the kept ones
-    [N] fp32.  The same numbers always give the same tokens, however the rows are batched."""
+    [N] fp32 (not differentiable: logits that require grad are refused while gradients are recorded).  The same numbers always
+    give the same tokens, however the rows are batched."""
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise _lib.LaedError("sample_rows: logits must be [N,V] with V >= 1, got %s" % (tuple(logits.shape),))
     code = _dtype_code(logits, "sample_rows")
-    if return_logp:
+    if return_logp:                                                # tokens have no derivative, their log-probabilities would
         _no_tangents("sample_rows", logits)
+        refuse_graph("sample_rows with return_logp", logits)
     N, V = logits.shape
     seed = offset = 0
     if (u is None) == (rng is None):

@@ -35,3 +35,21 @@ def test_forward_mode_derivatives_are_refused(ops):
         refused("CPU tensor", ops.dropout, z(4, 5), 0.5, (1, 0))
         refused("CPU tensor", ops.sample_rows, dual(3, 7), z(3))   # tokens have no derivative
     refused("CPU tensor", ops.gated_scan, z(2, 3, 4))
+
+
+def test_results_without_a_graph_are_refused_while_one_is_recorded(ops):
+    """The one-token forms and log-probabilities have no backward pass: inputs that require grad would be cut off in silence."""
+    from laed_amd.enc2dec.base_modules import GatedRNN
+    z = lambda *s: torch.zeros(*s, requires_grad=True)             # noqa: E731
+    c = torch.zeros
+    step = GatedRNN(5, 2).step
+    refused("no backward pass", ops.gated_scan_step, z(3, 4), c(3, 2))
+    refused("no backward pass", ops.gated_scan_step, c(3, 4), z(3, 2))
+    refused("no backward pass", ops.gated_scan_step, c(3, 4), c(3, 2), h_out=z(3, 2))
+    refused("no backward pass", step, z(3, 5), c(3, 2))
+    refused("no backward pass", step, c(3, 5), z(3, 2))
+    refused("no backward pass", ops.sample_rows, z(3, 7), c(3), return_logp=True)
+    refused("CPU tensor", ops.sample_rows, z(3, 7), c(3))          # tokens alone
+    with torch.no_grad():
+        refused("CPU tensor", ops.gated_scan_step, z(3, 4), z(3, 2))
+        refused("CPU tensor", ops.sample_rows, z(3, 7), c(3), return_logp=True)
