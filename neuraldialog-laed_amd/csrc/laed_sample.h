@@ -706,7 +706,8 @@ __device__ __forceinline__ bool draw_row(Shared& sh, const Who& w, const SampleA
     row.pow2 = sh.pow2;
     row.m = uniform(m);
     row.md = uniform((double)m);
-    row.c = uniform(fmin(STEPS * 1.4426950408889634074 / tau, 1e30));     // at 1e30 only equals of the largest one have a weight
+    row.c = uniform(fmin(STEPS * 1.4426950408889634074 / tau, 1e300));    // finite: 0 c is 0; floats differ by 1e-45 and more, so from
+                                                                           // 1e300 on only equals of the largest one have a weight
     row.per_step = uniform(tau * (0.693147180559945309417 / STEPS));
     row.tval = -INFINITY;
     row.tidx = -1;

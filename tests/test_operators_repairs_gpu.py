@@ -180,3 +180,17 @@ def test_forward_mode_through_a_backward_pass_is_refused(ops):
             assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].shape == leaf.shape
         with pytest.raises(RuntimeError, match="forward-mode"):
             ops.dropout(forward_ad.make_dual(x.detach(), torch.ones_like(x)), 0.5, (1, 2))
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# temperatures as small as the logits
+# ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [1e-20, 1e-30, 1e-41])
+def test_sample_tiny_temperatures_of_tiny_logits(ops, scale):
+    """What counts is the ratio: logits of 1e-30 under a temperature of 1e-30 (1e-41: subnormal ones) are far from equal."""
+    rows = (torch.randn(4, 3000, generator=torch.Generator().manual_seed(5), dtype=torch.float64) * scale).float()
+    for t in (0.3 * scale, scale, 5 * scale):
+        for kw in ({}, {"top_p": 0.9}, {"top_k": 700, "min_p": 0.03}, {"top_k": 50, "top_p": 0.8}):
+            sample_case(ops, rows, (0.2, 0.6, 0.95), temperature=t, **kw)
+    ids = ops.sample_rows(rows.cuda(), torch.full((4,), 0.9, device="cuda"), temperature=5e-324)      # the smallest number there is
+    assert torch.equal(ids.cpu(), rows.argmax(dim=1))
