@@ -388,7 +388,7 @@ int laed_gated_scan_bwd(const void* gi, int64_t gi_st, int64_t gi_sb, const floa
                         float* ws, int64_t ws_floats, void* stream);
 
 /* ------------------------------------------------------------------------------------------
- * Dropout without a stored mask: y = keep ? x / (1-p) : 0 (+ residual), keep(i) = draw offset + i of stream `seed` >= p,
+ * Dropout without a stored mask: y = keep ? x / (1-p) : 0 (+ residual), keep(i) = draw offset + i of stream `seed` >= (float)p,
  * i = row-major number of the element in the LOGICAL shape [d0][d1][d2] whatever the strides (the decision
  * laed_dropout_keep_mask puts at place i).  The backward pass is the same call on dy without a residual.  Strides of the
  * two outer dimensions in elements, the last one dense; residual may be NULL; y may be x or residual with the same strides.
@@ -396,7 +396,7 @@ int laed_gated_scan_bwd(const void* gi, int64_t gi_st, int64_t gi_sb, const floa
  * 64-bit numbers, used instead of the arguments (a captured graph draws new numbers when they are changed between replays).
  * ------------------------------------------------------------------------------------------ */
 int laed_dropout(const void* x, int64_t xs0, int64_t xs1, const void* residual, int64_t rs0, int64_t rs1,
-                 void* y, int64_t ys0, int64_t ys1, int64_t d0, int64_t d1, int64_t d2, int dtype, float p,
+                 void* y, int64_t ys0, int64_t ys1, int64_t d0, int64_t d1, int64_t d2, int dtype, double p,
                  uint64_t seed, uint64_t offset, const void* rng, void* stream);
 
 /* ------------------------------------------------------------------------------------------

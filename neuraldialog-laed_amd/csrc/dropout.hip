@@ -133,16 +133,18 @@ void dispatch(const DropArgs& a, hipStream_t stream) {
 }   // namespace
 
 extern "C" int laed_dropout(const void* x, int64_t xs0, int64_t xs1, const void* residual, int64_t rs0, int64_t rs1,
-                            void* y, int64_t ys0, int64_t ys1, int64_t d0, int64_t d1, int64_t d2, int dtype, float p,
+                            void* y, int64_t ys0, int64_t ys1, int64_t d0, int64_t d1, int64_t d2, int dtype, double p,
                             uint64_t seed, uint64_t offset, const void* rng, void* stream) {
     LAED_CHECK_ARG(d0 >= 0 && d1 >= 0 && d2 >= 0, "dropout: negative dimension");
-    LAED_CHECK_ARG(p >= 0.f && p <= 1.f, "dropout: p must lie in [0, 1]");
+    LAED_CHECK_ARG(p >= 0.0 && p <= 1.0, "dropout: p must lie in [0, 1]");
     LAED_CHECK_ARG(dtype >= LAED_F32 && dtype <= LAED_F16, "dropout: unknown dtype %d", dtype);
     if (d0 == 0 || d1 == 0 || d2 == 0) return 0;
     LAED_CHECK_ARG(x && y, "dropout: null pointer");
     LAED_CHECK_ARG(d0 <= (1ll << 40) / d1 / d2, "dropout: more than 2^40 elements");
-    DropArgs a = {x, residual, y, d0, d1, d2, xs0, xs1, rs0, rs1, ys0, ys1, p < 1.f ? (float)(1.0 / (1.0 - (double)p)) : 0.f,
-                  (unsigned)ceilf(p * 16777216.0f), seed, offset, (const uint64_t*)rng, 0, 0};
+    // the decision goes by p in fp32, as laed_dropout_keep_mask's; the factor by p itself: 1 / (1 - p) of the rounded p is off by
+    // 4 half steps of fp32 at p = 0.9 and by 16 at 0.99
+    DropArgs a = {x, residual, y, d0, d1, d2, xs0, xs1, rs0, rs1, ys0, ys1, p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f,
+                  (unsigned)ceilf((float)p * 16777216.0f), seed, offset, (const uint64_t*)rng, 0, 0};
 #define LAUNCH(T) dispatch<T>(a, (hipStream_t)stream)
     LAED_BY_DTYPE(dtype, LAUNCH);
 #undef LAUNCH

@@ -81,7 +81,7 @@ _SIGS = {
     "laed_gated_scan_fwd": ([_p, _i64, _i64, _p, _p, _i, _i, _i, _i, _i, _p, _i64, _i64, _p, _p, _p, _i64, _p], _i),
     "laed_gated_scan_bwd": ([_p, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _i, _i, _i, _i, _i, _p, _i64, _i64, _p,
                              _p, _i64, _p], _i),
-    "laed_dropout": ([_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i, _f, _u64, _u64, _p, _p], _i),
+    "laed_dropout": ([_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i, _d, _u64, _u64, _p, _p], _i),
     "laed_sample_rows": ([_p, _i64, _i64, _i, _i, _p, _u64, _u64, _d, _p, _i64, _p, _d, _p, _d, _p, _p, _p, _p], _i),
     "laed_adam_step": ([_p, _p, _p, _p, _i64, _i, _d, _d, _d, _d, _f, _p], _i),
     "laed_adam_step_multi": ([_i, _p, _p, _p, _p, _p, _i, _d, _d, _d, _d, _f, _p], _i),

@@ -194,3 +194,19 @@ def test_sample_tiny_temperatures_of_tiny_logits(ops, scale):
             sample_case(ops, rows, (0.2, 0.6, 0.95), temperature=t, **kw)
     ids = ops.sample_rows(rows.cuda(), torch.full((4,), 0.9, device="cuda"), temperature=5e-324)      # the smallest number there is
     assert torch.equal(ids.cpu(), rows.argmax(dim=1))
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# dropout's factor
+# ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("p", [0.6, 0.9, 0.99, 0.999, 1 - 1e-5])
+def test_dropout_factor_of_large_p(ops, p):
+    """1 / (1 - p) from p itself, not from p in fp32, forward and backward; the few that are kept decide by p in fp32."""
+    n = 1 << 20
+    x = torch.randn(n, device="cuda", requires_grad=True)
+    y = ops.dropout(x, p, (21, 4))
+    dy = torch.randn(n, device="cuda")
+    dx = torch.autograd.grad(y, x, dy)[0]
+    for got, src in ((y, x), (dx, dy)):
+        want, err, keep = F.dropout(f64(src), p, 21, 4)
+        assert keep.any() and (np.abs(f64(got) - want) <= err).all()
