@@ -93,7 +93,7 @@ class GatedRNN(nn.Module):
         super(GatedRNN, self).__init__()
         if not batch_first:
             raise NotImplementedError("laed_amd.GatedRNN: batch_first=True only, as laed_amd.GRU")
-        from ..nn_lib import Dropout
+        from ..nn_lib import Dropout, DropoutStream
         self.input_size, self.hidden_size, self.num_layers = input_size, hidden_size, num_layers
         self.batch_first, self.dropout, self.bidirectional = True, dropout, bidirectional
         self.suffixes = [''] + (['_reverse'] if bidirectional else [])
@@ -105,7 +105,8 @@ class GatedRNN(nn.Module):
         stdv = 1.0 / math.sqrt(hidden_size)
         for w in self.parameters():
             nn.init.uniform_(w, -stdv, stdv)
-        self.drop = nn.ModuleList(Dropout(dropout, seed=2468 + i) for i in range(num_layers - 1))
+        stream = DropoutStream()
+        self.drop = nn.ModuleList(Dropout(dropout, stream=stream, place=i) for i in range(num_layers - 1))
 
     def _gates(self, x_tm, layer, sfx=''):
         T, B, E = x_tm.shape

@@ -4,6 +4,9 @@ GumbelConnector / LinearConnector / GreedyConnector keep the reference signature
 Hidden2Discrete is the north star's name for the inline `q_y` Linear + view + log_softmax of
 sent_models.py:53,110-111.  Arithmetic runs in the HIP kernels (ops.py); there is no CPU path.
 """
+import itertools
+import weakref
+
 import torch
 import torch.nn as nn
 
@@ -42,17 +45,49 @@ class Embedding(nn.Embedding):
         return out.view(T, B, self.embedding_dim).transpose(0, 1)
 
 
+class DropoutStream(object):
+    """What tells the draws of a module without a seed of its own from all others': the lowest number that no living stream
+    holds, taken at the first draw.  So numbers go by the order in which a program's modules first draw -- alike on all ranks
+    of a job that run the same program -- and a model built anew, the old one gone, draws the old one's masks."""
+    held = weakref.WeakValueDictionary()          # number -> stream
+
+    def __init__(self):
+        self.number = None
+
+    def seed(self, place=0):
+        if self.number is None:
+            self.number = next(n for n in itertools.count() if n not in DropoutStream.held)
+            DropoutStream.held[self.number] = self
+        return 2468 + place + (self.number << 32)
+
+    def __deepcopy__(self, memo):
+        return DropoutStream() if self.number is None else self
+
+
 class Dropout(nn.Module):
     """Dropout drawn inside the kernel, forward and backward each from (seed, step): no mask in memory.  Every call draws the next
-    step's numbers, element i of the GLOBAL batch always the same ones: x is batch-first [B,...] (any strides), and a rank of a
-    data-parallel job draws from its rows' place on (equal shards).  residual: added to the result in the same kernel.  The step is
-    the host's number: a captured graph would repeat it (there, ops.dropout with its numbers on the device)."""
+    step's numbers (a recomputed forward pass is another call), element i of the GLOBAL batch always the same ones: x is
+    batch-first [B,...] (any strides), and a rank of a data-parallel job draws from its rows' place on (equal shards).  residual:
+    added to the result in the same kernel.  The step is the host's number: a captured graph would repeat it (there, ops.dropout
+    with its numbers on the device), and a resumed run sets it.
 
-    def __init__(self, p=0.5, seed=2468):
+    seed: None gives the module a stream of its own -- no two modules draw the same decisions; a copy of one that has drawn goes on
+    as the original does.  With a number, modules of the same seed draw the same.  stream, place: layers that share one stream."""
+
+    def __init__(self, p=0.5, seed=None, stream=None, place=0):
         super(Dropout, self).__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError("dropout probability has to be between 0 and 1, but got %r" % p)
-        self.p, self.seed, self.step = float(p), seed, 0
+        self.p, self.step = float(p), 0
+        self._seed, self.stream, self.place = seed, (DropoutStream() if stream is None else stream), place
+
+    @property
+    def seed(self):
+        return self.stream.seed(self.place) if self._seed is None else self._seed
+
+    @seed.setter
+    def seed(self, seed):
+        self._seed = seed
 
     def forward(self, x, residual=None):
         if not self.training or self.p == 0.0:
@@ -62,7 +97,7 @@ class Dropout(nn.Module):
         return ops.dropout(x, self.p, rng, residual=residual)
 
     def extra_repr(self):
-        return "p=%g, seed=%d" % (self.p, self.seed)
+        return "p=%g, seed=%s" % (self.p, self._seed)
 
 
 class LinearConnector(nn.Module):

@@ -53,3 +53,45 @@ def test_results_without_a_graph_are_refused_while_one_is_recorded(ops):
     with torch.no_grad():
         refused("CPU tensor", ops.gated_scan_step, z(3, 4), z(3, 2))
         refused("CPU tensor", ops.sample_rows, z(3, 7), c(3), return_logp=True)
+
+
+def test_modules_without_a_seed_draw_from_streams_of_their_own(ops, monkeypatch):
+    """(seed, offset) that each module hands to the operator: distinct between modules, layers and steps; unchanged for the first
+    stack of a program; given seeds are kept."""
+    import copy
+    import weakref
+    from laed_amd import nn_lib
+    from laed_amd.enc2dec.base_modules import GatedRNN
+    monkeypatch.setattr(nn_lib.DropoutStream, "held", weakref.WeakValueDictionary())
+    seen = []
+    monkeypatch.setattr(ops, "dropout", lambda x, p, rng, residual=None: seen.append(rng[0] & (2 ** 64 - 1)) or x)
+
+    def draws(m):
+        del seen[:]
+        for d in (m.drop if isinstance(m, GatedRNN) else [m]):
+            d(torch.zeros(2, 3))
+        return list(seen)
+
+    first, second = GatedRNN(4, 4, 4, dropout=0.5), GatedRNN(4, 4, 4, dropout=0.5)
+    a, b, twin = nn_lib.Dropout(), nn_lib.Dropout(), copy.deepcopy(second)
+    repr(first)                                                    # looking at a module takes no number
+    first.eval()
+    assert draws(first) == []
+    first.train()
+    assert draws(first) == [(2468 + i) * 1000003 for i in range(3)]
+    got = [draws(m) for m in (first, second, a, b, twin, second, a)]
+    assert got[0] == [(2468 + i) * 1000003 + 1 for i in range(3)]
+    flat = sum(got, [])
+    assert len(set(flat)) == len(flat)
+    later = copy.deepcopy(second)                                  # has drawn twice: goes on as the original does
+    assert draws(later) == draws(second)
+    held = second.drop[0].seed
+    del second
+    assert later.drop[0].seed == held and nn_lib.Dropout().seed not in (held, a.seed, b.seed)
+    assert draws(nn_lib.Dropout(0.5, seed=5)) == draws(nn_lib.Dropout(0.5, seed=5)) == [5 * 1000003]
+    a.seed = 7
+    a.step = 3
+    assert draws(a) == [7 * 1000003 + 3]
+    del first, later, b, twin                                      # built anew, the old ones gone: the same masks
+    anew = GatedRNN(4, 4, 4, dropout=0.5)
+    assert draws(anew) == [(2468 + i) * 1000003 for i in range(3)]

@@ -210,3 +210,21 @@ def test_dropout_factor_of_large_p(ops, p):
     for got, src in ((y, x), (dx, dy)):
         want, err, keep = F.dropout(f64(src), p, 21, 4)
         assert keep.any() and (np.abs(f64(got) - want) <= err).all()
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# modules
+# ----------------------------------------------------------------------------------------------------------------
+def test_two_modules_draw_different_masks():
+    """Two dropouts, and the dropouts inside two stacks of the same weights: independent decisions (kept by both: p^2 of them)."""
+    from laed_amd import nn_lib
+    from laed_amd.enc2dec.base_modules import GatedRNN
+    x, n = torch.ones(1 << 16, device="cuda"), 1 << 16
+    a, b = nn_lib.Dropout(0.5), nn_lib.Dropout(0.5)
+    both = float(((a(x) != 0) & (b(x) != 0)).double().mean())
+    assert abs(both - 0.25) < 5 * (0.25 * 0.75 / n) ** 0.5         # 5 standard deviations
+    stacks = [GatedRNN(6, 8, 2, dropout=0.5).cuda() for _ in range(2)]
+    stacks[1].load_state_dict(stacks[0].state_dict())
+    y = torch.randn(3, 9, 6, device="cuda")
+    assert not torch.equal(stacks[0](y)[0], stacks[1](y)[0])
+    assert torch.equal(stacks[0].eval()(y)[0], stacks[1].eval()(y)[0])
