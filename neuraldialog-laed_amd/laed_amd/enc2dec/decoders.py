@@ -214,7 +214,12 @@ class DecoderRNN(BaseRNN):
     def forward(self, batch_size, inputs=None, init_state=None, attn_context=None, mode=TEACH_FORCE,
                 gen_type='greedy', beam_size=4, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """gen_type='sample': temperature / top_k / top_p / min_p filter each step's distribution (ops.sample_rows; off by
-        default: Gumbel-max over the whole vocabulary, as the reference draws)."""
+        default: Gumbel-max over the whole vocabulary, as the reference draws).  Any other gen_type refuses them."""
+        filters = {'temperature': temperature, 'top_k': top_k, 'top_p': top_p, 'min_p': min_p}
+        if filters == {'temperature': 1.0, 'top_k': 0, 'top_p': 1.0, 'min_p': 0.0}:
+            filters = None
+        elif gen_type != 'sample':
+            raise ValueError("temperature, top_k, top_p and min_p belong to gen_type='sample'")
         ret_dict = dict()
         if mode == GEN:
             inputs = None
@@ -235,11 +240,6 @@ class DecoderRNN(BaseRNN):
         with torch.no_grad():
             h0 = init_state[0].detach().contiguous()
             sample = gen_type == 'sample'
-            filters = {'temperature': temperature, 'top_k': top_k, 'top_p': top_p, 'min_p': min_p}
-            if filters == {'temperature': 1.0, 'top_k': 0, 'top_p': 1.0, 'min_p': 0.0}:
-                filters = None
-            elif not sample:
-                raise ValueError("temperature, top_k, top_p and min_p belong to gen_type='sample'")
             u = None
             if sample and self.injected_u is not None:          # tests: replay recorded uniforms [max_len,B,V]
                 u = torch.as_tensor(self.injected_u, dtype=torch.float32).to(h0.device).contiguous()

@@ -95,3 +95,14 @@ def test_modules_without_a_seed_draw_from_streams_of_their_own(ops, monkeypatch)
     del first, later, b, twin                                      # built anew, the old ones gone: the same masks
     anew = GatedRNN(4, 4, 4, dropout=0.5)
     assert draws(anew) == [(2468 + i) * 1000003 for i in range(3)]
+
+
+@pytest.mark.parametrize("cell", ["gru", "glr"])
+@pytest.mark.parametrize("kw", [{"temperature": 0.5}, {"top_k": 3}, {"top_p": 0.9}, {"min_p": 0.1}])
+def test_filters_are_refused_where_nothing_is_drawn(cell, kw):
+    """Beam search, greedy decoding and teacher forcing would ignore them."""
+    from laed_amd.enc2dec.decoders import GEN, TEACH_FORCE, DecoderRNN
+    dec = DecoderRNN(11, 4, 5, 6, 2, 3, rnn_cell=cell)
+    for mode, gen_type in ((GEN, 'beam'), (GEN, 'greedy'), (TEACH_FORCE, 'greedy'), (TEACH_FORCE, 'beam')):
+        with pytest.raises(ValueError, match="belong to gen_type='sample'"):
+            dec(2, inputs=torch.zeros(2, 3, dtype=torch.int64), init_state=torch.zeros(1, 2, 6), mode=mode, gen_type=gen_type, **kw)
