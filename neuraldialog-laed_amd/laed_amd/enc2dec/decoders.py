@@ -97,7 +97,8 @@ class DecoderRNN(BaseRNN):
         # noise control for gen_type='sample' (gumbel_max, base_modules.py:54-67)
         self.sample_seed = 9876
         self.sample_step = 0
-        self.injected_u = None             # tests: uniforms [max_len,B,V] ([max_len,B] with filters) replayed instead of the RNG
+        # tests: uniforms [max_len,B,V] ([max_len,B] with filters, and always with rnn_cell='glr') replayed instead of the RNG
+        self.injected_u = None
 
     def _keep_mask_tm(self, B, T, device):
         """uint8 keep mask in time-major layout [T,B,E]; RNG keyed by the GLOBAL batch row."""
@@ -191,8 +192,11 @@ class DecoderRNN(BaseRNN):
         return decoder_outputs, h.unsqueeze(0), ret_dict
 
     def _generate_gated(self, h, sample, filters, u, seed, row0):
-        """Free-running decode of the gated linear recurrence, one token at a time: ids [L,B], states [L+1,B,H]."""
+        """Free-running decode of the gated linear recurrence, one token at a time: ids [L,B], states [L+1,B,H].  Sampling is
+        sample_rows' with filters and without: one uniform number a row and step, u [L,B] or number t * 2^32 + row0 + b."""
         B = h.shape[0]
+        if u is not None and tuple(u.shape) != (self.max_length, B):
+            raise ValueError("decode: u must be [max_len, B] = %s, got %s" % ((self.max_length, B), tuple(u.shape)))
         W, bias = self.project.weight.detach(), self.project.bias.detach()
         hbuf = torch.empty((self.max_length + 1,) + tuple(h.shape), device=h.device, dtype=torch.float32)
         hbuf[0].copy_(h)
@@ -214,7 +218,8 @@ class DecoderRNN(BaseRNN):
     def forward(self, batch_size, inputs=None, init_state=None, attn_context=None, mode=TEACH_FORCE,
                 gen_type='greedy', beam_size=4, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """gen_type='sample': temperature / top_k / top_p / min_p filter each step's distribution (ops.sample_rows; off by
-        default: Gumbel-max over the whole vocabulary, as the reference draws).  Any other gen_type refuses them."""
+        default: Gumbel-max over the whole vocabulary, as the reference draws, and with rnn_cell='glr' ops.sample_rows without a
+        filter).  Any other gen_type refuses them."""
         filters = {'temperature': temperature, 'top_k': top_k, 'top_p': top_p, 'min_p': min_p}
         if filters == {'temperature': 1.0, 'top_k': 0, 'top_p': 1.0, 'min_p': 0.0}:
             filters = None
@@ -241,7 +246,7 @@ class DecoderRNN(BaseRNN):
             h0 = init_state[0].detach().contiguous()
             sample = gen_type == 'sample'
             u = None
-            if sample and self.injected_u is not None:          # tests: replay recorded uniforms [max_len,B,V]
+            if sample and self.injected_u is not None:          # tests: replay recorded uniforms
                 u = torch.as_tensor(self.injected_u, dtype=torch.float32).to(h0.device).contiguous()
             seed, row0 = self.sample_seed * 1000003 + self.sample_step, parallel.rank() * batch_size
             ids, hbuf = self._generate_gated(h0, sample, filters, u, seed, row0) if gated else \

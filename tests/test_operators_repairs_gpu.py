@@ -228,3 +228,28 @@ def test_two_modules_draw_different_masks():
     y = torch.randn(3, 9, 6, device="cuda")
     assert not torch.equal(stacks[0](y)[0], stacks[1](y)[0])
     assert torch.equal(stacks[0].eval()(y)[0], stacks[1].eval()(y)[0])
+
+
+def test_unfiltered_sampling_of_the_gated_recurrence():
+    """rnn_cell='glr' without filters: sample_rows over the whole vocabulary, one uniform number a row and step; other shapes of
+    replayed numbers are refused."""
+    from laed_amd import ops
+    from laed_amd.enc2dec.decoders import GEN, DecoderRNN
+    torch.manual_seed(1)
+    V, E, H, B, L = 211, 8, 16, 5, 6
+    dec = DecoderRNN(V, L, E, H, 2, 3, rnn_cell='glr').cuda().eval()
+    with torch.no_grad():
+        dec.project.weight.mul_(8.0)
+    h0, u = torch.randn(1, B, H, device="cuda"), torch.rand(L, B)
+    for replayed in (u, None):
+        dec.injected_u, dec.sample_step = (None if replayed is None else u.numpy()), 3
+        lazy, _, ret = dec(B, init_state=h0, mode=GEN, gen_type='sample')
+        ids = torch.cat(ret[dec.KEY_SEQUENCE], dim=1).cpu().numpy()
+        logits = f64(ops.sgemm(lazy.h_tm.reshape(L * B, H).contiguous(), dec.project.weight.detach(), transB=True, bias=dec.project.bias.detach()))
+        for t in range(L):
+            n = replayed[t] if replayed is not None else ops.uniform(B, dec.sample_seed * 1000003 + 3, t << 32, "cuda").cpu()
+            assert ids[:, t].tolist() == [F.sample_row(logits[t * B + b], float(n[b]))[0] for b in range(B)], t
+    for shape in ((L, B, V), (L + 1, B), (L, B + 1)):
+        dec.injected_u = torch.rand(*shape).numpy()
+        with pytest.raises(ValueError, match="max_len, B"):
+            dec(B, init_state=h0, mode=GEN, gen_type='sample')
