@@ -253,3 +253,50 @@ def test_unfiltered_sampling_of_the_gated_recurrence():
         dec.injected_u = torch.rand(*shape).numpy()
         with pytest.raises(ValueError, match="max_len, B"):
             dec(B, init_state=h0, mode=GEN, gen_type='sample')
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# nothing is written beside an output
+# ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,B,H", [(1, 3, 5), (13, 2, 7), (65, 3, 33), (41, 2, 64), (1500, 2, 24), (1501, 1, 37)])
+def test_scan_does_not_write_beside_its_outputs(T, B, H, dt):
+    """The C entries on buffers with guards in front of, behind and (strided outputs) between the rows: out, dgi, hT, dh0, the tape
+    and the scratch.  The numbers are the 64-bit form's, to its bounds."""
+    from laed_amd._lib import check, lib, stream
+    code, pad, guard = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dt], 64, 7.0
+    ws_n, tape_n = int(lib.laed_gated_scan_workspace(T, B, H)), int(lib.laed_gated_scan_tape(T, B, H))
+    assert (ws_n > 0) == (T > 1000)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    gi = torch.randn(T, B, 2 * H, device="cuda", generator=g).to(dt)
+    h0 = torch.randn(B, H, device="cuda", generator=g)
+    dout, dhT = torch.randn(T, B, H, device="cuda", generator=g).to(dt), torch.randn(B, H, device="cuda", generator=g)
+    lengths = torch.tensor([T, T // 2, 0][:B], device="cuda")
+    for lens, reverse in ((None, 0), (lengths, 1)):
+        want = F.gated_scan(f64(gi), f64(h0), None if lens is None else lens.tolist(), bool(reverse), f64(dout), f64(dhT))
+        for gap, off in ((0, 0), (8, 0), (3, 1)):
+            def guarded(n, dtype=torch.float32):
+                buf = torch.full((n + 2 * pad + off,), guard, device="cuda", dtype=dtype)
+                return buf, buf[pad + off:pad + off + n]
+
+            def rows(width):                                       # [T][B][width] with `gap` elements behind each row
+                buf, mid = guarded(T * B * (width + gap), dt)
+                return buf, mid.view(T, B, width + gap)
+
+            (ob, o), (qb, q) = rows(H), rows(2 * H)
+            (tb, tape), (wb, ws) = guarded(tape_n), guarded(ws_n)
+            (hb, h), (db, d) = guarded(B * H), guarded(B * H)
+            at = lambda t: None if t is None else t.data_ptr()     # noqa: E731
+            scratch = (ws.data_ptr(), ws_n) if ws_n else (None, 0)
+            check(lib.laed_gated_scan_fwd(at(gi), B * 2 * H, 2 * H, at(h0), at(lens), T, B, H, code, reverse, at(o), B * (H + gap), H + gap,
+                                          at(h), at(tape), *scratch, stream()), "fwd")
+            check(lib.laed_gated_scan_bwd(at(gi), B * 2 * H, 2 * H, at(tape), at(lens), at(dout), B * H, H, at(dhT), T, B, H, code, reverse,
+                                          at(q), B * (2 * H + gap), 2 * H + gap, at(d), *scratch, stream()), "bwd")
+            for got, name in ((o[..., :H], "out"), (q[..., :2 * H], "dgi"), (h.view(B, H), "hT"), (d.view(B, H), "dh0")):
+                half = F.HALF_STEP[str(got.dtype).replace("torch.", "")]                 # one rounding to the output's type
+                tiny = 2.0 ** -25 if got.dtype == torch.float16 else 1e-38             # half of the smallest subnormal's place
+                bound = want[name + "_err"] + half * (np.abs(want[name]) + want[name + "_err"]) * 1.001 + tiny
+                assert (np.abs(f64(got) - want[name]) <= bound).all(), (name, gap, off)
+            assert (o[..., H:] == guard).all() and (q[..., 2 * H:] == guard).all()
+            for buf, n in ((ob, o.numel()), (qb, q.numel()), (tb, tape_n), (wb, ws_n), (hb, B * H), (db, B * H)):
+                assert (buf[:pad + off] == guard).all() and (buf[pad + off + n:] == guard).all()
