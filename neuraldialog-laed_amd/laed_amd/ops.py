@@ -1059,11 +1059,16 @@ def _seed_offset(rng, what):
     return int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF, None
 
 
+_INT = 2 ** 31 - 1        # sizes that the C entries take as 32-bit numbers: ctypes would pass the low 32 bits of a larger one
+
+
 def _scan_check(gi, h0, lengths):
     if gi.dim() != 3 or gi.shape[2] % 2:
         raise _lib.LaedError("gated_scan: gi must be [T,B,2H] (f | x), got %s" % (tuple(gi.shape),))
     _dtype_code(gi, "gated_scan")
     T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+    if T > _INT or B > _INT or H > _INT:
+        raise _lib.LaedError("gated_scan: T, B and H must be below 2^31, got %d, %d and %d" % (T, B, H))
     if h0 is not None and tuple(h0.shape) != (B, H):
         raise _lib.LaedError("gated_scan: h0 must be [B,H] = %s, got %s" % ((B, H), tuple(h0.shape)))
     if lengths is not None and (lengths.dim() != 1 or lengths.shape[0] != B or lengths.dtype.is_floating_point):
@@ -1161,6 +1166,8 @@ def gated_scan_step(gi, h, h_out=None):
     refuse_graph("gated_scan_step", gi, h, h_out)
     code = _dtype_code(gi, "gated_scan_step")
     B, H = gi.shape[0], gi.shape[1] // 2
+    if B > _INT or H > _INT:
+        raise _lib.LaedError("gated_scan_step: B and H must be below 2^31, got %d and %d" % (B, H))
     for t, name in ((h, "h"), (h_out, "h_out")):
         if t is not None and (t.dtype != torch.float32 or t.shape != (B, H) or not t.is_contiguous()):
             raise _lib.LaedError("gated_scan_step: %s must be a contiguous fp32 [B,H] state" % name)
@@ -1295,6 +1302,8 @@ def sample_rows(logits, u=None, rng=None, temperature=1.0, top_k=0, top_p=1.0, m
         _no_tangents("sample_rows", logits)
         refuse_graph("sample_rows with return_logp", logits)
     N, V = logits.shape
+    if V > _INT:
+        raise _lib.LaedError("sample_rows: V must be below 2^31, got %d" % V)
     seed = offset = 0
     if (u is None) == (rng is None):
         raise _lib.LaedError("sample_rows: either u or rng = (seed, offset) is needed")

@@ -106,3 +106,13 @@ def test_filters_are_refused_where_nothing_is_drawn(cell, kw):
     for mode, gen_type in ((GEN, 'beam'), (GEN, 'greedy'), (TEACH_FORCE, 'greedy'), (TEACH_FORCE, 'beam')):
         with pytest.raises(ValueError, match="belong to gen_type='sample'"):
             dec(2, inputs=torch.zeros(2, 3, dtype=torch.int64), init_state=torch.zeros(1, 2, 6), mode=mode, gen_type=gen_type, **kw)
+
+
+def test_sizes_beyond_32_bits_are_refused(ops):
+    """Expanded tensors reach them in little memory; the C entries would see the low 32 bits."""
+    n, z = 2 ** 32 + 5, torch.zeros
+    refused("must be below 2.31", ops.gated_scan, z(1, 1, 2).expand(1, n, 2))
+    refused("must be below 2.31", ops.gated_scan, z(1, 1, 2).expand(n, 1, 2))
+    refused("must be below 2.31", ops.gated_scan, z(1, 1, 1).expand(1, 1, 2 * n))
+    refused("must be below 2.31", ops.gated_scan_step, z(1, 2).expand(n, 2), z(1, 1).expand(n, 1))
+    refused("must be below 2.31", ops.sample_rows, z(1, 1).expand(1, n), z(1))
