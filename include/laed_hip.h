@@ -373,7 +373,7 @@ int laed_tanh_bwd(const float* y, const float* dy, float* dx, int64_t n, void* s
  * dimension dense.  gi, out, dout, dgi have the type `dtype`; states (h0, hT, dhT, dh0: [B][H]) are fp32, may be NULL (h0 /
  * dhT: zeros; hT / dh0: not wanted).  lengths (may be NULL): positions t >= lengths[b] are identity steps -- not read, out and
  * dgi are zeros there, the state passes (a length <= 0: hT = h0; > T: T).  reverse != 0 runs from t = T-1 down to 0.
- * T = 0 copies h0 to hT.  hT may be h0 (in place).  tape (may be NULL: no backward pass follows): laed_gated_scan_tape
+ * T = 0 copies h0 to hT; H <= 2^28.  hT may be h0 (in place).  tape (may be NULL: no backward pass follows): laed_gated_scan_tape
  * floats written by the forward and read by the backward call, which runs the steps again from it.  ws: scratch of
  * laed_gated_scan_workspace floats, 16-byte aligned (0: none is needed, NULL) -- few channels and many steps are split over time.
  * ------------------------------------------------------------------------------------------ */

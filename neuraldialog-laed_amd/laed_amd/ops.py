@@ -1021,8 +1021,9 @@ def _no_tangents(what, *ts):
 
 def refuse_graph(what, *ts):
     """Results that no backward pass can reach are refused for inputs that ask for one."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise _lib.LaedError("%s has no backward pass: call it under torch.no_grad() or with detached tensors" % what)
+    for t in ts:                                                   # no generator: this is a part of a 12 us call
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise _lib.LaedError("%s has no backward pass: call it under torch.no_grad() or with detached tensors" % what)
 
 
 # the current stream's handle as a number: torch.cuda.current_stream() builds a Stream object, 3 us of a 15 us call (15 us in
@@ -1163,7 +1164,7 @@ def gated_scan_step(gi, h, h_out=None):
     if gi.dim() != 2 or gi.shape[1] % 2:
         raise _lib.LaedError("gated_scan_step: gi must be [B,2H] (f | x), got %s" % (tuple(gi.shape),))
     _no_tangents("gated_scan_step", gi, h)
-    refuse_graph("gated_scan_step", gi, h, h_out)
+    refuse_graph("gated_scan_step", gi, h, None if h_out is h else h_out)
     code = _dtype_code(gi, "gated_scan_step")
     B, H = gi.shape[0], gi.shape[1] // 2
     if B > _INT or H > _INT:

@@ -116,3 +116,13 @@ def test_sizes_beyond_32_bits_are_refused(ops):
     refused("must be below 2.31", ops.gated_scan, z(1, 1, 1).expand(1, 1, 2 * n))
     refused("must be below 2.31", ops.gated_scan_step, z(1, 2).expand(n, 2), z(1, 1).expand(n, 1))
     refused("must be below 2.31", ops.sample_rows, z(1, 1).expand(1, n), z(1))
+
+
+def test_channels_that_no_grid_holds_are_refused():
+    """One sequence's threads, H times the waves of a block, have to fit a grid (H <= 2^28 always does)."""
+    from laed_amd._lib import lib
+    one = 16 << 20
+    assert lib.laed_gated_scan_fwd(one, 0, 0, None, None, 57, 1, 2 ** 29, 1, 0, one, 0, 0, None, None, None, 0, None) == -1
+    assert b"H too large" in lib.laed_last_error()
+    assert lib.laed_gated_scan_bwd(one, 0, 0, one, None, None, 0, 0, None, 9, 1, 2 ** 31 - 1, 1, 0, one, 0, 0, None, None, 0, None) == -1
+    assert b"H too large" in lib.laed_last_error()

@@ -142,25 +142,30 @@ def test_dropout_lengths_around_a_block(ops):
             assert torch.equal(ops.dropout(x, 0.5, (3, 4)), torch.where(keep, x * 2, torch.zeros_like(x))), (n, dt)
 
 
-def test_scan_more_channels_than_a_grid_holds(ops):
-    """2^21 sequences x 2049 channels of one bf16 input expanded over the batch, one channel a thread: 2^32 threads and more.
-    Forward and backward; every sequence gives the numbers of a call of four."""
-    if not spare_memory(100):
-        pytest.skip("needs 100 GB of device memory")
-    B, H = 1 << 21, 2049
+@pytest.mark.parametrize("T,B,H,gib", [(1, 1 << 21, 2049, 100), (65, 209700, 2049, 190)])
+def test_scan_more_channels_than_a_grid_holds(ops, T, B, H, gib):
+    """One bf16 input expanded over the batch, one channel a thread: more than 2^31 threads, so two or three launches (T = 65: with
+    two tiles on each one's tape).  Forward and backward; every sequence gives the numbers of a call of four."""
+    if not spare_memory(gib):
+        pytest.skip("needs %d GB of device memory" % gib)
     g = torch.Generator(device="cuda").manual_seed(3)
-    gi = torch.randn(1, 1, 2 * H, device="cuda", generator=g).bfloat16()
-    few = gi.expand(1, 4, 2 * H).contiguous().requires_grad_(True)
+    gi = torch.randn(T, 1, 2 * H, device="cuda", generator=g).bfloat16()
+    dout = torch.randn(T, 1, H, device="cuda", generator=g).bfloat16()
+    few = gi.expand(T, 4, 2 * H).contiguous().requires_grad_(True)
     want, wantT = ops.gated_scan(few)
-    dwant = torch.autograd.grad(want, few, torch.ones_like(want))[0]
-    x = gi.expand(1, B, 2 * H).requires_grad_(True)
+    dwant = torch.autograd.grad(want, few, dout.expand(T, 4, H))[0]
+    x = gi.expand(T, B, 2 * H).requires_grad_(True)
     out, hT = ops.gated_scan(x)
-    assert torch.equal(want[0, :1], want[0, 3:]) and torch.equal(dwant[0, :1], dwant[0, 3:])
-    same = lambda a, b: all(bool((a[i:i + (1 << 18)] == b).all()) for i in range(0, B, 1 << 18))   # noqa: E731
-    assert same(out[0], want[0, 0]) and same(hT, wantT[0])
+    assert torch.equal(want[:, :1], want[:, 3:]) and torch.equal(dwant[:, :1], dwant[:, 3:])
+
+    def same(a, b):
+        step = max(1, (1 << 29) // (a.shape[0] * a.shape[2]))
+        return all(bool((a[:, i:i + step] == b[:, :1]).all()) for i in range(0, B, step))
+
+    assert same(out, want) and same(hT[None], wantT[None])
     del hT
-    d = torch.autograd.grad(out, x, torch.ones(1, 1, H, device="cuda", dtype=torch.bfloat16).expand(1, B, H))[0]
-    assert same(d[0], dwant[0, 0])
+    d = torch.autograd.grad(out, x, dout.expand(T, B, H))[0]
+    assert same(d, dwant)
     del out, d, x
     torch.cuda.empty_cache()
 
