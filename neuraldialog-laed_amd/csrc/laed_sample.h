@@ -476,7 +476,8 @@ __device__ __forceinline__ u64 block_sum(Shared& sh, const Who& w, u64 mine) {
 
 // More than CAP candidates in a bin (equal logits, or a tail that the linear bins do not reach): bisection over the ordered
 // bit patterns between the bin's smallest and largest value, one pass each (at most 32), then the equal ones in vocabulary
-// order.  Rare: each pass costs what the histogram's does.
+// order.  Each pass costs what the histogram's does.  Rare in fp32; in 16 bits a long vocabulary's tail is full of equal
+// logits (64 rows of 100000 bf16 under top-p 0.9: 197 us, 33 under a temperature alone).
 template <bool MASS, typename R>
 __device__ __forceinline__ void bisect(Shared& sh, const Who& w, Row& row, R& walk, u64 need) {
     unsigned lo = (unsigned)sh.kmin, hi = (unsigned)sh.kmax;
@@ -777,9 +778,13 @@ void go(SampleArgs a, hipStream_t stream) {
 template <typename T>
 void launch(const SampleArgs& a, hipStream_t stream) {
     const int64_t nvec = (a.V + 2 * (16 / sizeof(T)) - 2) / (16 / sizeof(T));      // the row's start may lie inside a vector
-    // The row in registers, as few vectors a thread as hold it (13 beside 16: 52 registers leave room, 64 spill a little).
-    // 256 threads per row where they hold it and rows are many: several rows share a CU and overlap their phases; a few
-    // rows are done sooner by 1024.
+    // The row in registers, as few vectors a thread as hold it.  Up to 8 of them nothing is spilled; 13 spill 28 registers (fp32; 53
+    // in 16 bits), 16 spill 171 (238 to 241).  fp32 rows of 50000, 64 and 1024 of them under top-p 0.9: 13 vectors 39 and 173 us, 16
+    // 53 and 274, the row read again in every pass 53 and 237.  Rows that only 16 hold: 60000 fp32 52 and 294 us, read again
+    // 60 and 267; 128003 bf16 under a temperature 43 and 217 us, read again 45 and 205.
+    // 256 threads per row where they hold it and rows are many: several rows share a CU and overlap their phases (2000 fp32, top-p:
+    // 4096 rows 68 us against 186 with 1024 threads).  Fewer than 256 rows get 1024 threads, which has turned out to be
+    // a little slower too (64 rows 12.9 us against 11.6).
     if (nvec <= 512 && (a.N >= 256 || nvec <= 256)) go<T, Held<T, 2>, 256>(a, stream);
     else if (nvec <= 1024 * 4) go<T, Held<T, 4>, 1024>(a, stream);
     else if (nvec <= 1024 * 8) go<T, Held<T, 8>, 1024>(a, stream);

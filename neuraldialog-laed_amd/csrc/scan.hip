@@ -54,8 +54,15 @@ ScanPlan scan_plan(int T, int B, int H) {
     if (p.waves < 1) p.waves = 1;
     p.tiles = (int)cdiv64(T, p.waves * LSTEP);
     // blocks of 64 x 2 channels; 1024 of them are four (with 4 channels a lane, two) per CU: against 512, the long case's
-    // passes took 29 and 37 us instead of 41 and 49.  From 512 strips on the channels alone keep the CUs busy, and a
-    // second read of the inputs would only cost.
+    // passes took 29 and 37 us instead of 41 and 49.  From 512 strips on one segment, which reads the inputs once.  Forward + backward
+    // in us, one segment | this rule's number (inputs not in the caches):
+    //   strips   bf16 T 1024   bf16 T 4096   fp32 T 1024   fp32 T 4096
+    //       64    231 |  96     926 |  226    148 | 104     597 |  333
+    //      128    247 | 119     988 |  428    165 | 155     644 |  604
+    //      256    267 | 216    1055 |  809    221 | 321     813 | 1179
+    //      511    399 | 536    1551 | 2054    515 | 738    2246 | 2944
+    // So the border of 512 is right for neither type: 16 bits gain up to 256 strips, fp32 up to 128, and between there and
+    // 512 the second read costs more than the blocks gain.
     const int64_t strips = cdiv64((int64_t)B * H, 128);
     int64_t segs = strips >= 512 ? 1 : cdiv64(1024, strips);
     if (segs > p.tiles / 2) segs = p.tiles / 2;                    // a segment is two tiles at least: its block folds, then scans
