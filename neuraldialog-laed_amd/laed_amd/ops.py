@@ -271,6 +271,8 @@ def decode_greedy(emb, w_ih, w_hh, b_ih, b_hh, proj_w, proj_b, h0, max_len, go_i
     """Free-running decode from h0 [B,H]: greedy, or (sample=True) Gumbel-max sampling with replayed uniforms
     u [max_len,B,V] or the counter RNG keyed by (seed, step, row0 + row).  filters: dict of sample_rows' temperature, top_k,
     top_p, min_p -- each symbol is then drawn by sample_rows' rule from one uniform number, u [max_len,B] or the counter RNG."""
+    if filters is not None and not sample:
+        raise ValueError("decode: filters belong to sample=True")
     B, H = h0.shape
     V, E = emb.shape
     dev = h0.device

@@ -126,3 +126,9 @@ def test_channels_that_no_grid_holds_are_refused():
     assert b"H too large" in lib.laed_last_error()
     assert lib.laed_gated_scan_bwd(one, 0, 0, one, None, None, 0, 0, None, 9, 1, 2 ** 31 - 1, 1, 0, one, 0, 0, None, None, 0, None) == -1
     assert b"H too large" in lib.laed_last_error()
+
+
+def test_filters_of_a_greedy_decode_loop_are_refused(ops):
+    w = [torch.zeros(*s) for s in ((11, 5), (18, 5), (18, 6), (18,), (18,), (11, 6), (11,), (2, 6))]
+    with pytest.raises(ValueError, match="belong to sample=True"):
+        ops.decode_greedy(*w, 4, 2, filters={"top_k": 3})
